@@ -43,7 +43,8 @@ typedef enum mfk_activation {
     MFK_ACT_NONE = 0,
     MFK_ACT_RELU = 1,
     MFK_ACT_GELU = 2,
-    MFK_ACT_GELU_TANH = 3
+    MFK_ACT_GELU_TANH = 3,
+    MFK_ACT_SILU = 4 /* v / (1 + exp(-v)); the gated feed-forward block only */
 } mfk_activation;
 
 /* Tensor-core arithmetic for the fp32 GEMMs. 3xTF32 splits each operand into tf32 hi + lo and
@@ -335,6 +336,77 @@ int mfk_dot_f32(const float* x, const float* y, int64_t n, float* out, void* str
  * device gives a device-to-device copy. */
 int mfk_copy_peer(void* dst, int32_t dst_device, const void* src, int32_t src_device,
                   int64_t bytes, void* stream);
+
+/* The gated feed-forward block and its backward pass, in fp32:
+ *     gate = x w_gate, up = x w_up, h = act(gate) * up, y = h w_down.
+ * x is rows x d, w_gate and w_up d x f, w_down f x d; element (i, j) of a matrix at
+ * p[i*rs + j*cs], and of each matrix's two strides one must be 1 (MFK_ERR_UNSUPPORTED otherwise;
+ * weights stored [outputs, inputs] have rs = 1). w_gate and w_up must lie the same way round.
+ * activation is any mfk_activation. No counterpart in the reference, which composes such blocks
+ * from gemm and elementwise calls; like mfk_gemm_f32's 3xTF32 form the products are
+ * fp32-faithful: each matrix is split into fp16 (hi, lo) pairs under one power-of-two scale per
+ * 128 x 128 block, three products are summed, and sums are held in fp32 over any depth. An entry
+ * keeps 22 bits or more while it is within 2^-17 of the largest entry of its block, and an
+ * absolute error of 2^-39 of that entry below. A non-finite operand entry makes the results that
+ * depend on it non-finite (an infinity may come out as NaN).
+ *
+ * mfk_gated_ffn_f32: y has row stride ldy >= d. saved (optional, 16-byte aligned,
+ * mfk_gated_ffn_saved_floats(rows, f) floats of device memory) receives gate and up for the
+ * backward pass, in the kernels' own order.
+ *
+ * mfk_gated_ffn_backward_f32: from grad = dL/dy the gradients
+ *     dh = grad w_down^T, dgate = dh * up * act'(gate), dup = dh * act(gate),
+ *     dx = dgate w_gate^T + dup w_up^T, dw_gate = x^T dgate, dw_up = x^T dup, dw_down = h^T grad.
+ * saved: what the forward call with the same x, w_gate, w_up left, or NULL (recomputed). dx may be
+ * NULL, and the three weight gradients may be NULL together. dw_gate and dw_up share their
+ * strides; of each output's strides one must be 1. The gradients are written, not added to, and
+ * must not overlap the inputs or each other. rows = 0 gives zero weight gradients.
+ *
+ * Both take their workspace from the stream-ordered allocator. */
+typedef struct mfk_gated_ffn_desc {
+    const float* x;
+    int64_t x_rs, x_cs;
+    const float* w_gate;
+    int64_t w_gate_rs, w_gate_cs;
+    const float* w_up;
+    int64_t w_up_rs, w_up_cs;
+    const float* w_down;
+    int64_t w_down_rs, w_down_cs;
+    int64_t rows, d, f;
+    int32_t activation; /* mfk_activation */
+    int32_t reserved;   /* 0 */
+} mfk_gated_ffn_desc;
+
+typedef struct mfk_gated_ffn_grads {
+    const float* grad;
+    int64_t grad_rs, grad_cs;
+    float* dx;
+    int64_t ld_dx;
+    float* dw_gate;
+    float* dw_up;
+    int64_t dw_rs, dw_cs;
+    float* dw_down;
+    int64_t dw_down_rs, dw_down_cs;
+} mfk_gated_ffn_grads;
+
+int mfk_gated_ffn_f32(const mfk_gated_ffn_desc* desc, float* y, int64_t ldy, float* saved,
+                      void* stream);
+int64_t mfk_gated_ffn_saved_floats(int64_t rows, int64_t f);
+int mfk_gated_ffn_backward_f32(const mfk_gated_ffn_desc* desc, const mfk_gated_ffn_grads* grads,
+                               const float* saved, void* stream);
+
+/* Orthogonalises an update by Newton-Schulz products: x = u / (||u||_F + eps), then `steps` times
+ *     x <- a x + (b g + c g g) x,  g = x x^T
+ * (on the transpose where rows > cols, so that g is the smaller Gram matrix), for each of `batch`
+ * matrices of rows x cols: u at update + i*batch_stride with row stride row_stride and unit column
+ * stride (any row stride), the result at out + i*out_batch_stride with row stride ld >= cols. out
+ * must not overlap update. steps >= 1, eps >= 0 (a zero matrix with eps = 0 gives NaN). The norm
+ * is summed in double; the products are computed as in mfk_gated_ffn_f32. No counterpart in the
+ * reference. */
+int mfk_orthogonalize_f32(const float* update, int64_t batch, int64_t rows, int64_t cols,
+                          int64_t row_stride, int64_t batch_stride, float* out, int64_t ld,
+                          int64_t out_batch_stride, int32_t steps, float a, float b, float c,
+                          float eps, void* stream);
 
 /* Process-wide precision used when a descriptor says MFK_PRECISION_DEFAULT. The reference's
  * public signatures have no precision argument, so its adapters leave the default in place. */

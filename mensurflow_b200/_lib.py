@@ -1,7 +1,7 @@
 """Loader for the sm_100a kernel library (``lib/libmfkernels.so``, C ABI in ``include/mfk.h``).
 
 There is no fallback: if the library is missing or fails to load, every op raises. The
-structures below mirror ``mfk_gemm_desc`` / ``mfk_batch_desc`` field for field.
+structures below mirror the descriptors of ``mfk.h`` field for field.
 """
 from __future__ import annotations
 
@@ -24,7 +24,7 @@ MFK_ERR_SCRATCH_LIMIT = 7
 NOALLOC_SCRATCH_BYTES = 64 * 1024 * 1024
 IPC_HANDLE_BYTES = 64
 
-ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH = 0, 1, 2, 3
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = 0, 1, 2, 3, 4
 PRECISION_DEFAULT, PRECISION_3XTF32, PRECISION_1XTF32 = -1, 0, 1
 BINARY_ADD, BINARY_SUB, BINARY_MUL, BINARY_DIV = 0, 1, 2, 3
 
@@ -57,6 +57,10 @@ EXPORTED = (
     "mfk_binary_f32",
     "mfk_scal_f32",
     "mfk_dot_f32",
+    "mfk_gated_ffn_f32",
+    "mfk_gated_ffn_saved_floats",
+    "mfk_gated_ffn_backward_f32",
+    "mfk_orthogonalize_f32",
     "mfk_set_default_precision",
     "mfk_get_default_precision",
     "mfk_device_status",
@@ -89,6 +93,28 @@ class BatchDesc(ctypes.Structure):
         ("a_offsets", ctypes.c_void_p), ("b_offsets", ctypes.c_void_p),
         ("a_stride", ctypes.c_int64), ("b_stride", ctypes.c_int64),
         ("c_in_stride", ctypes.c_int64), ("c_stride", ctypes.c_int64),
+    ]
+
+
+class GatedFfnDesc(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("x_rs", ctypes.c_int64), ("x_cs", ctypes.c_int64),
+        ("w_gate", ctypes.c_void_p), ("w_gate_rs", ctypes.c_int64), ("w_gate_cs", ctypes.c_int64),
+        ("w_up", ctypes.c_void_p), ("w_up_rs", ctypes.c_int64), ("w_up_cs", ctypes.c_int64),
+        ("w_down", ctypes.c_void_p), ("w_down_rs", ctypes.c_int64), ("w_down_cs", ctypes.c_int64),
+        ("rows", ctypes.c_int64), ("d", ctypes.c_int64), ("f", ctypes.c_int64),
+        ("activation", ctypes.c_int32), ("reserved", ctypes.c_int32),
+    ]
+
+
+class GatedFfnGrads(ctypes.Structure):
+    _fields_ = [
+        ("grad", ctypes.c_void_p), ("grad_rs", ctypes.c_int64), ("grad_cs", ctypes.c_int64),
+        ("dx", ctypes.c_void_p), ("ld_dx", ctypes.c_int64),
+        ("dw_gate", ctypes.c_void_p), ("dw_up", ctypes.c_void_p),
+        ("dw_rs", ctypes.c_int64), ("dw_cs", ctypes.c_int64),
+        ("dw_down", ctypes.c_void_p), ("dw_down_rs", ctypes.c_int64),
+        ("dw_down_cs", ctypes.c_int64),
     ]
 
 
@@ -157,6 +183,13 @@ def lib() -> ctypes.CDLL:
             so.mfk_binary_f32.argtypes = [i32, vp, vp, vp, i64, vp]
             so.mfk_scal_f32.argtypes = [f32, vp, vp, i64, vp]
             so.mfk_dot_f32.argtypes = [vp, vp, i64, vp, vp]
+            so.mfk_gated_ffn_f32.argtypes = [ctypes.POINTER(GatedFfnDesc), vp, i64, vp, vp]
+            so.mfk_gated_ffn_saved_floats.argtypes = [i64, i64]
+            so.mfk_gated_ffn_saved_floats.restype = i64
+            so.mfk_gated_ffn_backward_f32.argtypes = [ctypes.POINTER(GatedFfnDesc),
+                                                      ctypes.POINTER(GatedFfnGrads), vp, vp]
+            so.mfk_orthogonalize_f32.argtypes = [vp, i64, i64, i64, i64, i64, vp, i64, i64, i32,
+                                                 f32, f32, f32, f32, vp]
             so.mfk_set_default_precision.argtypes = [i32]
             so.mfk_get_default_precision.restype = i32
             so.mfk_device_status.argtypes = [ctypes.POINTER(ctypes.c_uint32), i32]

@@ -1,0 +1,223 @@
+"""Operators of language models, on B200 tensors: the gated feed-forward block with its backward
+pass and the orthogonalised update, beside ``linear`` and ``linear_backward``.
+
+They follow the package's manner: fp32 CUDA tensors, work queued on the current stream of the
+tensors' device, explicit backward functions, ``ValueError`` for bad arguments and
+``NotImplementedError`` where there is no kernel. Views with a unit stride in either of a matrix's
+two dimensions (row-major, transposed, sliced) go to the kernels as they are; others are packed
+first. The reference has no counterpart of these operators (it composes blocks from gemm and
+elementwise calls).
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Sequence
+
+import torch
+
+from . import _lib
+from ._lib import GatedFfnDesc, GatedFfnGrads, check
+from .ops import _kernel_for, _require, _same, _stream, contiguous
+
+_GATED_ACTS = {None: _lib.ACT_NONE, "none": _lib.ACT_NONE, "relu": _lib.ACT_RELU,
+               "gelu": _lib.ACT_GELU, "gelu_tanh": _lib.ACT_GELU_TANH, "silu": _lib.ACT_SILU}
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return t.data_ptr() if t is not None and t.numel() else None
+
+
+def _lies(t: torch.Tensor) -> Optional[bool]:
+    """False: rows are contiguous, True: columns are, None: neither."""
+    if t.stride(1) == 1 or t.shape[1] <= 1:
+        return False
+    return True if t.stride(0) == 1 or t.shape[0] <= 1 else None
+
+
+def _unit(t: torch.Tensor) -> torch.Tensor:
+    """t itself when one of its strides is 1, else a packed copy."""
+    return contiguous(t) if _lies(t) is None else t
+
+
+def _strides(t: torch.Tensor):
+    """Strides for the kernels: a dimension of one entry has none that matters."""
+    rows, cols = t.shape
+    cs = 1 if cols <= 1 else t.stride(1)
+    rs = max(cols, 1) if rows <= 1 and cs == 1 else t.stride(0)
+    return rs, cs
+
+
+class GatedSaved:
+    """What ``gated_ffn(..., save=True)`` keeps for the backward pass: the gate's and the up
+    projection's results, in the kernels' own order, in a device tensor (``buffer``)."""
+
+    def __init__(self, buffer: torch.Tensor, rows: int, features: int):
+        self.buffer = buffer
+        self.rows = rows
+        self.features = features
+
+
+def _gated_args(op, x, w_gate, w_up, w_down, activation, transpose_w):
+    _require(x, op, "x", 1, at_least=True)
+    for t, name in ((w_gate, "w_gate"), (w_up, "w_up"), (w_down, "w_down")):
+        _require(t, op, name, 2)
+    _same(op, x, w_gate, w_up, w_down)
+    if activation not in _GATED_ACTS:
+        raise ValueError(f"{op}: unknown activation {activation!r}")
+    gate, up, down = (t.t() if transpose_w else t for t in (w_gate, w_up, w_down))
+    d, f = gate.shape
+    if x.shape[-1] != d:
+        raise ValueError(f"{op}: x {tuple(x.shape)} does not fit w_gate {tuple(w_gate.shape)}")
+    if tuple(up.shape) != (d, f):
+        raise ValueError(f"{op}: w_up {tuple(w_up.shape)} differs from w_gate "
+                         f"{tuple(w_gate.shape)}")
+    if tuple(down.shape) != (f, d):
+        raise ValueError(f"{op}: w_down {tuple(w_down.shape)} does not fit w_gate "
+                         f"{tuple(w_gate.shape)}")
+    _kernel_for(op, x)
+    rows = 1
+    for s in x.shape[:-1]:
+        rows *= s
+    x2 = _rows_of(x, rows, d)
+    gate, up, down = _unit(gate), _unit(up), _unit(down)
+    if _lies(gate) != _lies(up):  # the two projections share a tile: one way round
+        gate, up = contiguous(gate), contiguous(up)
+    desc = GatedFfnDesc()
+    desc.x = _ptr(x2)
+    desc.x_rs, desc.x_cs = _strides(x2)
+    desc.w_gate, desc.w_up, desc.w_down = _ptr(gate), _ptr(up), _ptr(down)
+    desc.w_gate_rs, desc.w_gate_cs = _strides(gate)
+    desc.w_up_rs, desc.w_up_cs = _strides(up)
+    desc.w_down_rs, desc.w_down_cs = _strides(down)
+    desc.rows, desc.d, desc.f = rows, d, f
+    desc.activation = _GATED_ACTS[activation]
+    return desc, (x2, gate, up, down)
+
+
+def _rows_of(t: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
+    """t [..., cols] as a matrix [rows, cols] with a unit stride: a view where there is one."""
+    if t.dim() == 2:
+        return _unit(t)
+    if t.numel() and not t.is_contiguous():
+        try:
+            return _unit(t.view(rows, cols))
+        except RuntimeError:
+            t = contiguous(t)
+    return t.reshape(rows, cols)
+
+
+def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
+              activation: Optional[str] = "silu", *, transpose_w: bool = False,
+              save: bool = False):
+    """(act(x @ w_gate) * (x @ w_up)) @ w_down: the gated feed-forward block. x is [..., d],
+    w_gate and w_up are [d, f], w_down is [f, d]; with ``transpose_w`` the weights are stored
+    [outputs, inputs], as in ``linear``. ``activation``: "silu", "gelu" (exact), "gelu_tanh",
+    "relu" or None. Both projections, the activation and their product are one kernel; its result
+    never leaves the split form the down projection reads.
+
+    With ``save`` the result is (y, saved): ``saved`` spares ``gated_ffn_backward`` the two
+    projections at the price of 8 bytes per row and feature.
+
+    The products are fp32-faithful (fp16 pairs under one power-of-two scale per 128 x 128 block,
+    sums in fp32), whatever ``set_default_precision`` says; an entry more than 2^17 below the
+    largest of its block keeps an absolute error of 2^-39 of that largest one. Non-finite inputs
+    give non-finite results, though an infinity may come out as NaN."""
+    desc, keep = _gated_args("gated_ffn", x, w_gate, w_up, w_down, activation, transpose_w)
+    rows, d, f = desc.rows, desc.d, desc.f
+    with torch.cuda.device(x.device):
+        y = torch.empty(tuple(x.shape), dtype=torch.float32, device=x.device)
+        saved = None
+        if save:
+            size = _lib.lib().mfk_gated_ffn_saved_floats(rows, f)
+            saved = GatedSaved(torch.empty(size, dtype=torch.float32, device=x.device), rows, f)
+        check(_lib.lib().mfk_gated_ffn_f32(ctypes.byref(desc), _ptr(y), max(d, 1),
+                                           _ptr(saved.buffer) if save else None, _stream()),
+              "gated_ffn")
+    return (y, saved) if save else y
+
+
+def gated_ffn_backward(grad: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor,
+                       w_up: torch.Tensor, w_down: torch.Tensor,
+                       activation: Optional[str] = "silu", *, saved: Optional[GatedSaved] = None,
+                       transpose_w: bool = False, need_x: bool = True, need_w: bool = True):
+    """(dx, dw_gate, dw_up, dw_down) of ``gated_ffn`` for grad = dL/dy, with the forward call's
+    arguments; dx has x's shape and the weights' gradients have the weights' own layouts.
+    ``saved`` from the forward call with the same x and weights; without it the two projections
+    are computed again. What is not needed is None."""
+    op = "gated_ffn_backward"
+    desc, keep = _gated_args(op, x, w_gate, w_up, w_down, activation, transpose_w)
+    _require(grad, op, "grad")
+    _same(op, x, grad)
+    if tuple(grad.shape) != tuple(x.shape):
+        raise ValueError(f"{op}: grad {tuple(grad.shape)} differs from x {tuple(x.shape)}")
+    rows, d, f = desc.rows, desc.d, desc.f
+    if saved is not None:
+        if not isinstance(saved, GatedSaved):
+            raise TypeError(f"{op}: saved must come from gated_ffn(..., save=True)")
+        if (saved.rows, saved.features) != (rows, f) or saved.buffer.device != x.device:
+            raise ValueError(f"{op}: saved belongs to another call ({saved.rows} rows, "
+                             f"{saved.features} features)")
+    if not need_x and not need_w:
+        return None, None, None, None
+    with torch.cuda.device(x.device):
+        g2 = _rows_of(grad, rows, d)
+        o = GatedFfnGrads()
+        o.grad = _ptr(g2)
+        o.grad_rs, o.grad_cs = _strides(g2)
+        dx = dw_gate = dw_up = dw_down = None
+        if need_x:
+            dx = torch.empty(tuple(x.shape), dtype=torch.float32, device=x.device)
+            o.dx, o.ld_dx = _ptr(dx), max(d, 1)
+        if need_w:
+            dw_gate, dw_up, dw_down = (torch.empty(tuple(t.shape), dtype=torch.float32,
+                                                   device=x.device)
+                                       for t in (w_gate, w_up, w_down))
+            o.dw_gate, o.dw_up, o.dw_down = _ptr(dw_gate), _ptr(dw_up), _ptr(dw_down)
+            o.dw_rs, o.dw_cs = (1, max(d, 1)) if transpose_w else (max(f, 1), 1)
+            o.dw_down_rs, o.dw_down_cs = (1, max(f, 1)) if transpose_w else (max(d, 1), 1)
+        check(_lib.lib().mfk_gated_ffn_backward_f32(
+            ctypes.byref(desc), ctypes.byref(o), _ptr(saved.buffer) if saved else None,
+            _stream()), op)
+    return dx, dw_gate, dw_up, dw_down
+
+
+def orthogonalize(update: torch.Tensor, steps: int = 5,
+                  coefficients: Sequence[float] = (3.4445, -4.7750, 2.0315),
+                  eps: float = 1e-7) -> torch.Tensor:
+    """The update with its singular values drawn towards 1 by Newton-Schulz products: for each
+    matrix of ``update`` [..., m, n], x = u / (||u||_F + eps), then ``steps`` times
+    x <- a x + (b g + c g g) x with g = x x^T and (a, b, c) = ``coefficients`` (on the transpose
+    where m > n). All matrices of a batch run in the same launches. The Gram matrix and its square
+    are symmetric: only their lower halves are computed. Arithmetic as in ``gated_ffn``."""
+    op = "orthogonalize"
+    _require(update, op, "update", 2, at_least=True)
+    if not isinstance(steps, int) or isinstance(steps, bool) or steps < 1:
+        raise ValueError(f"{op}: steps must be a whole number of at least 1, got {steps!r}")
+    if len(coefficients) != 3:
+        raise ValueError(f"{op}: coefficients must be (a, b, c)")
+    if not eps >= 0:
+        raise ValueError(f"{op}: eps must be at least 0, got {eps!r}")
+    _kernel_for(op, update)
+    m, n = update.shape[-2:]
+    if update.numel() == 0:
+        return torch.empty(tuple(update.shape), dtype=torch.float32, device=update.device)
+    with torch.cuda.device(update.device):
+        if update.stride(-1) != 1 and n > 1 and (update.stride(-2) == 1 or m <= 1):
+            return orthogonalize(update.transpose(-2, -1), steps, coefficients,
+                                 eps).transpose(-2, -1)
+        u = update
+        if n > 1 and u.stride(-1) != 1:
+            u = contiguous(u)
+        try:
+            u = u.view(-1, m, n)
+        except RuntimeError:
+            u = contiguous(u).view(-1, m, n)
+        out = torch.empty(tuple(update.shape), dtype=torch.float32, device=update.device)
+        batch = u.shape[0]
+        a, b, c = (float(v) for v in coefficients)
+        check(_lib.lib().mfk_orthogonalize_f32(u.data_ptr(), batch, m, n,
+                                               u.stride(1) if m > 1 else n,
+                                               u.stride(0) if batch > 1 else 0, out.data_ptr(),
+                                               n, m * n, steps, a, b, c, float(eps), _stream()),
+              op)
+    return out

@@ -24,6 +24,7 @@
 #include "movement.cuh"
 #include "prep.cuh"
 #include "simt.cuh"
+#include "split_mm.cuh"
 
 // A B operand split once (mfk_pack_b_f32): op(B) as K-major panels [n][kp] of tf32 values, hi
 // and (3xTF32) lo, in device memory the handle owns.
@@ -1563,6 +1564,8 @@ int mfk_copy_peer(void* dst, int32_t dst_device, const void* src, int32_t src_de
 }
 
 }  // extern "C"
+
+#include "split_host.cuh"
 
 extern "C" {
 

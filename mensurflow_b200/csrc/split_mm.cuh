@@ -1,0 +1,963 @@
+// fp32 matrix products on the fp16 tensor cores, for the language-model operators (the gated
+// feed-forward block and its backward pass, the orthogonalised update).
+//
+// Mathematics. A matrix is cut into blocks of 128 x 128. With s the power of two that brings a
+// block's largest magnitude into [2^14, 2^15), each entry x of the block is held as two halves,
+//     hi = fp16(s x),  lo = fp16(s x - hi),
+// so s x = hi + lo to 2^-23 of itself (and never worse than 2^-40 of the block's largest entry:
+// lo's spacing ends at 2^-24). A product of two such matrices takes three fp16 products,
+//     (s_a a)(s_b b) ~ lo hi + hi lo + hi hi,
+// summed in fp32; the term left out, lo lo, is below 2^-22 of the product. fp16 tensor products
+// run at twice the tf32 rate, so this is twice as fast as a tf32 three-way split of the same 22
+// bits; the price is the block scale.
+//
+// Accumulation. tcgen05 rounds its fp32 accumulator toward zero on every instruction: each one
+// loses about 3.4e-8 of the running sum, always towards zero (measured: 3.8e-6 relative to the
+// result after 192 instructions, 1.2e-5 after 3072 spread over stream-K parts). So a tensor-memory accumulator
+// only ever holds one 128-deep chunk (24 instructions, the small lo products of a stage first),
+// and the epilogue warps add the chunks, scaled by the two blocks' 1/s, in fp32 registers with
+// round to nearest.
+//
+// Layout. A block is 64 KB: hi then lo, each as 16 columns-of-eight ("lines"), a line holding
+// 128 rows x 8 halves (16 bytes a row, 2 KB). 8 rows x 16 bytes are one core matrix of the
+// unswizzled operand layouts, and the same bytes serve as a K-major operand (contraction along
+// the stored columns) and as an MN-major one (along the stored rows): no operand is ever
+// transposed or split twice. The epilogues write blocks with full 128-byte rows of 16-byte
+// stores, one per lane.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "mfk_ptx.cuh"
+
+namespace mfk {
+
+constexpr int kXBlk = 128;                 // block side
+constexpr int kXBlockBytes = 65536;        // hi 32 KB, lo 32 KB
+constexpr int kXLineBytes = 2048;          // 128 rows x 8 halves
+constexpr int kXBlockLines = 32;
+constexpr int kXThreads = 320;             // TMA warp, MMA warp, eight epilogue warps
+constexpr int kXEpiWarp0 = 2;
+constexpr int kXEpiThreads = 256;
+
+enum XEpi : int { kXF32 = 0, kXSplit = 1, kXGated = 2, kXGatedBwd = 3 };
+
+// A split matrix as an operand: block (mn, k) of matrix z.
+struct XOperand {
+    int line0;        // first line of block 0 in the tensor maps
+    int ldb;          // blocks per stored block row
+    int bstride;      // blocks from one matrix of a batch to the next
+    int flip;         // 0: contraction along the stored columns, 1: along the stored rows
+    int sym;          // symmetric: only blocks (i, j) with i >= j are stored
+    const float* inv; // 1/s per block
+};
+
+struct XOut {
+    uint8_t* data;
+    float* inv;
+    int ldb, bstride;
+};
+
+struct XArgs {
+    XOperand a[2], b[2];   // two segments of the contraction, or (gated) b = gate and up
+    int kc0, kc;           // chunks of 128 in segment 0, in all
+    int last0, last1;      // stages of 64 in each segment's last chunk (1 or 2)
+    int mb, nb;            // output blocks
+    int m, n;              // output entries
+    int tiles_m, tiles_n, splits, units, sym;
+    int tiles;             // per matrix
+    float alpha, beta;     // acc * alpha + C * beta
+    XOut c;                // C as a split matrix (beta != 0)
+    float* out;            // fp32 output, row stride ld, batch stride out_bs
+    long long ld, out_bs;
+    XOut o[3];             // split outputs: result / h; dgate, dup, h
+    float* gate;           // saved pre-activations in accumulator order (null: not saved)
+    float* up;
+    float* gmax;           // largest |gate|, |up| per block
+    int act;
+    int store_h;
+    float* part;           // partial accumulators of split contractions
+    int* count;
+};
+
+// ---- PTX forms this kernel adds --------------------------------------------------------------
+
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar,
+                                            int32_t x, int32_t y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_2d_cg2(void* dst, const CUtensorMap* map,
+                                                uint32_t bar_cluster_addr, int32_t x, int32_t y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster_addr), "r"(x), "r"(y)
+        : "memory");
+}
+
+template <int CG>
+__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                        uint32_t idesc, uint32_t accumulate) {
+    if constexpr (CG == 1) {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+            : "memory");
+    } else {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+            : "memory");
+    }
+}
+
+// 32 lanes x 16 consecutive columns, landed when it returns.
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+          "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+
+// kind::f16 with fp16 operands and an fp32 accumulator (fields as idesc_tf32; formats 0 = F16).
+__host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool a_mn_major, bool b_mn_major) {
+    return (1u << 4) | ((a_mn_major ? 1u : 0u) << 15) | ((b_mn_major ? 1u : 0u) << 16) |
+           ((static_cast<uint32_t>(n) >> 3) << 17) | ((static_cast<uint32_t>(m) >> 4) << 24);
+}
+
+__device__ __forceinline__ void epi_bar() {
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+}
+
+// ---- the split -------------------------------------------------------------------------------
+
+// s (a power of two) for a block whose largest finite magnitude is amax, and 1/s. s stays a
+// normal number with a normal reciprocal: below 2^-112 the scaled values merely get smaller.
+__device__ __forceinline__ void split_scale(float amax, float& s, float& inv) {
+    const int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;  // amax >= 0
+    const int sh = amax == 0.0f ? 0 : min(14 - e, 126);
+    s = __uint_as_float(static_cast<uint32_t>(sh + 127) << 23);
+    inv = __uint_as_float(static_cast<uint32_t>(127 - sh) << 23);
+}
+
+__device__ __forceinline__ float finite_abs(float x) {
+    const float a = fabsf(x);
+    return a <= 3.402823466e38f ? a : 0.0f;  // infinities and NaN do not set a block's scale
+}
+
+// (hi, lo) of two scaled values, packed. A non-finite value goes into hi alone.
+__device__ __forceinline__ void split_pair(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x0, x1);
+    const float2 hf = __half22float2(h);
+    const float l0 = fabsf(x0) <= 65504.0f ? x0 - hf.x : 0.0f;
+    const float l1 = fabsf(x1) <= 65504.0f ? x1 - hf.y : 0.0f;
+    const __half2 l = __floats2half2_rn(l0, l1);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// Eight consecutive columns (16-byte line `chunk`) of one row of a block.
+__device__ __forceinline__ void store_split8(uint8_t* block, int chunk, int row, const float* v,
+                                             float s) {
+    uint4 h, l;
+    split_pair(v[0] * s, v[1] * s, h.x, l.x);
+    split_pair(v[2] * s, v[3] * s, h.y, l.y);
+    split_pair(v[4] * s, v[5] * s, h.z, l.z);
+    split_pair(v[6] * s, v[7] * s, h.w, l.w);
+    uint8_t* p = block + chunk * kXLineBytes + row * 16;
+    *reinterpret_cast<uint4*>(p) = h;
+    *reinterpret_cast<uint4*>(p + kXBlockBytes / 2) = l;
+}
+
+struct XSource {
+    const float* src;      // rows x cols, unit column stride
+    long long rs, bs;      // row stride, batch stride (elements)
+    int rows, cols, batch;
+    int rb, cb;            // blocks
+    int vec;               // every row starts on 16 bytes
+    int first;             // index of this matrix's first block in the launch
+    uint8_t* data;
+    float* inv;
+    double* sumsq;         // per-block sum of squares, or null
+};
+
+constexpr int kXMaxSources = 5;
+struct XSources {
+    XSource s[kXMaxSources];
+    int count;
+};
+
+// One 128 x 128 block per CTA of 256 threads: 64 entries per thread in registers, the block's
+// largest magnitude, then hi and lo. Lanes take 8 rows x 4 eight-column lines, so a warp reads
+// 128-byte row pieces and writes whole 128-byte core matrices. Bound by HBM: 4 bytes read, 4
+// written per entry.
+__global__ void __launch_bounds__(256) split_blocks_kernel(const __grid_constant__ XSources list) {
+    int which = 0;
+#pragma unroll
+    for (int i = 1; i < kXMaxSources; ++i)
+        if (i < list.count && static_cast<int>(blockIdx.x) >= list.s[i].first) which = i;
+    const XSource& t = list.s[which];
+    const int local = static_cast<int>(blockIdx.x) - t.first;
+    const int per = t.rb * t.cb;
+    const int z = local / per;
+    const int ij = local - z * per;
+    const int bi = ij / t.cb, bj = ij - bi * t.cb;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int r8 = lane >> 2, c4 = lane & 3;
+    const float* base = t.src + z * t.bs;
+    float v[2][4][8];
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+        const int row = bi * kXBlk + (warp * 2 + a) * 8 + r8;
+        const bool row_ok = row < t.rows;
+        const float* p = base + static_cast<long long>(row_ok ? row : 0) * t.rs;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int col = bj * kXBlk + (b * 4 + c4) * 8;
+#pragma unroll
+            for (int j = 0; j < 8; j += 4) {
+                float4 q = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (row_ok) {
+                    if (t.vec && col + j + 4 <= t.cols) {
+                        q = *reinterpret_cast<const float4*>(p + col + j);
+                    } else {
+                        if (col + j < t.cols) q.x = p[col + j];
+                        if (col + j + 1 < t.cols) q.y = p[col + j + 1];
+                        if (col + j + 2 < t.cols) q.z = p[col + j + 2];
+                        if (col + j + 3 < t.cols) q.w = p[col + j + 3];
+                    }
+                }
+                v[a][b][j] = q.x;
+                v[a][b][j + 1] = q.y;
+                v[a][b][j + 2] = q.z;
+                v[a][b][j + 3] = q.w;
+            }
+        }
+    }
+    float amax = 0.0f;
+    double sum = 0.0;
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) amax = fmaxf(amax, finite_abs(v[a][b][j]));
+    if (t.sumsq != nullptr) {
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    sum += static_cast<double>(v[a][b][j]) * static_cast<double>(v[a][b][j]);
+    }
+    __shared__ uint32_t wmax[8];
+    __shared__ double wsum[8];
+    const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(amax));
+    if (t.sumsq != nullptr) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
+    if (lane == 0) {
+        wmax[warp] = m;
+        wsum[warp] = sum;
+    }
+    __syncthreads();
+    uint32_t all = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) all = max(all, wmax[w]);
+    float s, inv;
+    split_scale(__uint_as_float(all), s, inv);
+    if (threadIdx.x == 0) {
+        t.inv[local] = inv;
+        if (t.sumsq != nullptr) {
+            double total = 0.0;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) total += wsum[w];
+            t.sumsq[local] = total;
+        }
+    }
+    uint8_t* block = t.data + static_cast<long long>(local) * kXBlockBytes;
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+            store_split8(block, b * 4 + c4, (warp * 2 + a) * 8 + r8, v[a][b], s);
+}
+
+// Divides matrix z of a batch by its Frobenius norm (+ eps) by scaling the blocks' 1/s: exact up
+// to the factor's own rounding, since every 1/s is a power of two. The blocks' sums of squares
+// are added in one fixed order, in double.
+__global__ void __launch_bounds__(256) split_normalize_kernel(const double* sumsq, float* inv,
+                                                              int blocks, float eps) {
+    __shared__ double part[256];
+    const double* p = sumsq + static_cast<long long>(blockIdx.x) * blocks;
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < blocks; i += 256) sum += p[i];
+    part[threadIdx.x] = sum;
+    __syncthreads();
+#pragma unroll
+    for (int o = 128; o > 0; o >>= 1) {
+        if (static_cast<int>(threadIdx.x) < o) part[threadIdx.x] += part[threadIdx.x + o];
+        __syncthreads();
+    }
+    const float f = static_cast<float>(1.0 / (sqrt(part[0]) + static_cast<double>(eps)));
+    float* q = inv + static_cast<long long>(blockIdx.x) * blocks;
+    for (int i = threadIdx.x; i < blocks; i += 256) q[i] *= f;
+}
+
+// ---- activations of the gated block ----------------------------------------------------------
+
+enum XAct : int { kXActNone = 0, kXActRelu = 1, kXActGelu = 2, kXActGeluTanh = 3, kXActSilu = 4 };
+
+// act(v) and act'(v) in fp32. silu and the tanh form of GELU go through the logistic function
+// s(z) = 1 / (1 + exp(-z)): 0.5 (1 + tanh z) = s(2 z).
+__device__ __forceinline__ float2 act_slope(float v, int act) {
+    if (act == kXActSilu) {
+        const float s = __frcp_rn(1.0f + expf(-v));
+        return make_float2(v * s, s * (1.0f + v * (1.0f - s)));
+    }
+    if (act == kXActRelu) return v > 0.0f ? make_float2(v, 1.0f) : make_float2(v == v ? 0.0f : v, 0.0f);
+    if (act == kXActGelu) {
+        const float phi = 0.5f * erfcf(v * -0.70710678118654752f);
+        return make_float2(v * phi, phi + v * (0.39894228040143268f * expf(-0.5f * v * v)));
+    }
+    if (act == kXActGeluTanh) {
+        const float w = fminf(fmaxf(v, -16.0f), 16.0f);  // the logistic is 0 or 1 beyond
+        const float z2 = 1.5957691216057308f * (w + 0.044715f * w * w * w);
+        const float s = __frcp_rn(1.0f + expf(-z2));
+        const float dz2 = 1.5957691216057308f * (1.0f + 0.134145f * w * w);
+        return make_float2(v * s, s + w * s * (1.0f - s) * dz2);
+    }
+    return make_float2(v, 1.0f);
+}
+
+// The largest |act'| over all inputs (GELU's is 1.1290): bounds the gate's gradient.
+constexpr float kXMaxSlope = 1.13f;
+
+// ---- the product -----------------------------------------------------------------------------
+
+template <int CG, int NB>
+struct XConfig {
+    static constexpr int kBBlocks = CG == 2 ? 1 : NB;   // blocks of B this CTA loads
+    static constexpr int kStageBytes = 32768 * (1 + kBBlocks);
+    static constexpr int kStages = kBBlocks == 2 ? 2 : 3;
+    static constexpr int kTmemCols = NB * 256;          // two accumulators
+    static constexpr int kStageArea = kStages * kStageBytes;
+    static constexpr int kEpiBytes = 8 * 4096;          // 32 x 32 floats per epilogue warp
+    static constexpr int kSmemBytes = kStageArea + kEpiBytes + 1024 + 512;
+};
+
+struct XUnit {
+    int z, tm, tn, s, c0, c1, tile;
+};
+
+__device__ __forceinline__ XUnit x_unit(const XArgs& g, int u) {
+    XUnit w;
+    const int t = u / g.splits;
+    w.s = u - t * g.splits;
+    w.tile = t;
+    w.z = t / g.tiles;
+    int q = t - w.z * g.tiles;
+    if (g.sym) {  // lower triangle, row by row
+        int i = static_cast<int>((sqrtf(8.0f * static_cast<float>(q) + 1.0f) - 1.0f) * 0.5f);
+        while (i * (i + 1) / 2 > q) --i;
+        while ((i + 1) * (i + 2) / 2 <= q) ++i;
+        w.tm = i;
+        w.tn = q - i * (i + 1) / 2;
+    } else {  // bands of eight tile rows, column by column, so the operands in flight stay in L2
+        const int band = q / (8 * g.tiles_n);
+        const int first = band * 8;
+        const int height = min(8, g.tiles_m - first);
+        q -= first * g.tiles_n;
+        w.tn = q / height;
+        w.tm = first + q - w.tn * height;
+    }
+    w.c0 = static_cast<int>(static_cast<long long>(g.kc) * w.s / g.splits);
+    w.c1 = static_cast<int>(static_cast<long long>(g.kc) * (w.s + 1) / g.splits);
+    return w;
+}
+
+// Whether a tile whose first block along the operand's mn is `mn0` reads chunk k along the
+// blocks' stored rows (MN-major). A symmetric matrix stores only its lower blocks: a chunk right
+// of the tile's first block comes from (k, mn), transposed. All blocks of one MMA agree: for
+// k > mn0 every block of the tile has mn <= k or is one below (k >= mn0 + 1), and a diagonal
+// block reads either way.
+__device__ __forceinline__ int x_flip(const XOperand& o, int mn0, int k) {
+    return o.sym ? (k > mn0 ? 1 : 0) : o.flip;
+}
+
+__device__ __forceinline__ int x_block(const XOperand& o, int z, int mn, int k, int flip) {
+    return z * o.bstride + (flip ? k * o.ldb + mn : mn * o.ldb + k);
+}
+
+// The 128 x 64 (or 64 x 128) half of a block that stage `half` of a chunk reads: hi, then lo.
+template <int CG>
+__device__ __forceinline__ void x_load(uint8_t* dst, const CUtensorMap* mk, const CUtensorMap* mm,
+                                       uint64_t* bar, uint32_t bar0, const XOperand& o, int z,
+                                       int mn0, int mn, int k, int half) {
+    const int flip = x_flip(o, mn0, k);
+    const int line = o.line0 + x_block(o, z, mn, k, flip) * kXBlockLines;
+    const CUtensorMap* map = flip ? mm : mk;
+    const int x = flip ? half * 128 : 0;           // rows 64 half.. of every line (8-byte units)
+    const int y = flip ? line : line + half * 8;   // lines 8 half..
+    if constexpr (CG == 1) {
+        tma_load_2d(dst, map, bar, x, y);
+        tma_load_2d(dst + 16384, map, bar, x, y + 16);
+    } else {
+        tma_load_2d_cg2(dst, map, bar0, x, y);
+        tma_load_2d_cg2(dst + 16384, map, bar0, x, y + 16);
+    }
+}
+
+template <int CG, int NB, int EPI>
+__device__ __forceinline__ void x_producer(const XArgs& g, const CUtensorMap* mk,
+                                           const CUtensorMap* mm, uint8_t* stages, uint64_t* full,
+                                           uint64_t* empty, uint32_t rank, int first, int step) {
+    using C = XConfig<CG, NB>;
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int u = first; u < g.units; u += step) {
+        const XUnit w = x_unit(g, u);
+        const int i = min(w.tm * CG + static_cast<int>(rank), g.mb - 1);
+        for (int c = w.c0; c < w.c1; ++c) {
+            const int seg = EPI == kXF32 && c >= g.kc0 ? 1 : 0;
+            const int k = seg ? c - g.kc0 : c;
+            const int halves = c == g.kc0 - 1 ? g.last0 : (c == g.kc - 1 ? g.last1 : 2);
+            for (int h = 0; h < halves; ++h) {
+                if (!mbar_wait(&empty[stage], phase ^ 1u, 1u << 0)) {
+                    // the copies in flight land before this CTA may leave
+                    const uint64_t t0 = global_timer();
+                    while (global_timer() - t0 < 1000000ull) {
+                    }
+                    return;
+                }
+                uint8_t* s = stages + stage * C::kStageBytes;
+                uint32_t bar0 = 0;
+                if constexpr (CG == 1) {
+                    mbar_arrive_expect_tx(&full[stage], C::kStageBytes);
+                } else {
+                    if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * C::kStageBytes);
+                    bar0 = mapa_shared(&full[stage], 0);
+                }
+                x_load<CG>(s, mk, mm, &full[stage], bar0, g.a[seg], w.z, w.tm * CG, i,
+                           k, h);
+#pragma unroll
+                for (int b = 0; b < C::kBBlocks; ++b) {
+                    const int bb = CG == 2 ? static_cast<int>(rank) : b;
+                    if constexpr (EPI == kXGated) {
+                        x_load<CG>(s + 32768 * (1 + b), mk, mm, &full[stage], bar0, g.b[bb], w.z,
+                                   w.tn, w.tn, k, h);
+                    } else {
+                        x_load<CG>(s + 32768 * (1 + b), mk, mm, &full[stage], bar0, g.b[seg], w.z,
+                                   w.tn * NB, min(w.tn * NB + bb, g.nb - 1), k, h);
+                    }
+                }
+                if (++stage == C::kStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+    }
+}
+
+// One lane of the (pair's first) CTA.
+template <int CG, int NB, int EPI>
+__device__ __forceinline__ void x_mma(const XArgs& g, uint32_t tmem, uint8_t* stages,
+                                      uint64_t* full, uint64_t* empty, uint64_t* tfull,
+                                      uint64_t* tempty, int first, int step) {
+    using C = XConfig<CG, NB>;
+    constexpr int kM = 128 * CG;
+    constexpr int kN = CG == 2 ? 128 * NB : 128;
+    int stage = 0, buf = 0;
+    uint32_t phase = 0, tphase = 0;
+    const uint32_t stage0 = smem_u32(stages);
+    for (int u = first; u < g.units; u += step) {
+        const XUnit w = x_unit(g, u);
+        const int i = w.tm * CG, j = EPI == kXGated ? w.tn : w.tn * NB;
+        for (int c = w.c0; c < w.c1; ++c) {
+            const int seg = EPI == kXF32 && c >= g.kc0 ? 1 : 0;
+            const int k = seg ? c - g.kc0 : c;
+            const int halves = c == g.kc0 - 1 ? g.last0 : (c == g.kc - 1 ? g.last1 : 2);
+            const int fa = x_flip(g.a[seg], i, k), fb = x_flip(g.b[seg], j, k);
+            // K-major: core matrices 2 KB apart along k, 128 B along rows; 16 deep = two lines.
+            // MN-major (a line keeps 64 rows, 1 KB): 128 B apart along k, 1 KB along the other.
+            const uint32_t a_lbo = fa ? 128u : 2048u, a_sbo = fa ? 1024u : 128u;
+            const uint32_t b_lbo = fb ? 128u : 2048u, b_sbo = fb ? 1024u : 128u;
+            const uint32_t a_step = fa ? 256u : 4096u, b_step = fb ? 256u : 4096u;
+            const uint32_t idesc = idesc_f16(kM, kN, fa != 0, fb != 0);
+            if (!mbar_wait(&tempty[buf], tphase ^ 1u, 1u << 1)) return;
+            tc_fence_after();
+            const uint32_t d = tmem + static_cast<uint32_t>(buf * NB * 128);
+            for (int h = 0; h < halves; ++h) {
+                if (!mbar_wait(&full[stage], phase, 1u << 1)) return;
+                tc_fence_after();
+                const uint32_t sa = stage0 + stage * C::kStageBytes;
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) {
+                    const uint64_t ah = smem_desc(sa + ks * a_step, a_lbo, a_sbo, kSwizzleNone);
+                    const uint64_t al =
+                        smem_desc(sa + 16384 + ks * a_step, a_lbo, a_sbo, kSwizzleNone);
+#pragma unroll
+                    for (int b = 0; b < C::kBBlocks; ++b) {
+                        const uint32_t sb = sa + 32768 * (1 + b) + ks * b_step;
+                        const uint64_t bh = smem_desc(sb, b_lbo, b_sbo, kSwizzleNone);
+                        const uint64_t bl = smem_desc(sb + 16384, b_lbo, b_sbo, kSwizzleNone);
+                        mma_f16<CG>(d + b * 128, al, bh, idesc, (h | ks) ? 1u : 0u);
+                        mma_f16<CG>(d + b * 128, ah, bl, idesc, 1u);
+                    }
+                }
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) {
+                    const uint64_t ah = smem_desc(sa + ks * a_step, a_lbo, a_sbo, kSwizzleNone);
+#pragma unroll
+                    for (int b = 0; b < C::kBBlocks; ++b) {
+                        const uint32_t sb = sa + 32768 * (1 + b) + ks * b_step;
+                        mma_f16<CG>(d + b * 128, ah,
+                                    smem_desc(sb, b_lbo, b_sbo, kSwizzleNone), idesc, 1u);
+                    }
+                }
+                if constexpr (CG == 1) {
+                    mma_commit(&empty[stage]);
+                } else {
+                    mma_commit_cg2_mc(&empty[stage], 3);
+                }
+                if (++stage == C::kStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+            if constexpr (CG == 1) {
+                mma_commit(&tfull[buf]);
+            } else {
+                mma_commit_cg2_mc(&tfull[buf], 3);
+            }
+            if (++buf == 2) {
+                buf = 0;
+                tphase ^= 1u;
+            }
+        }
+    }
+}
+
+// The largest of a value over the epilogue's threads, in a shared slot. Three sets of slots take
+// turns: before a tile's barrier the next tile's set is cleared, which was last read before the
+// barrier of the tile before.
+__device__ __forceinline__ void x_max_into(uint32_t* red, float amax) {
+    const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(amax));
+    if ((threadIdx.x & 31) == 0) atomicMax(red, m);
+}
+
+// Thread (quarter q, half h, lane) owns row 32 q + lane of the CTA's 128 and, of every 128-column
+// block of the tile, columns 64 h .. 64 h + 63: acc[64 b + j] is column 64 h + j of block b.
+template <int CG, int NB, int EPI>
+__device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* epi_smem, uint32_t* red,
+                                           int* last_flag, uint32_t tmem, uint64_t* tfull,
+                                           uint64_t* tempty, uint32_t rank, int first, int step) {
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int q = warp % 4, half = (warp - kXEpiWarp0) / 4;
+    const int row = q * 32 + lane;
+    const int et = threadIdx.x - kXEpiWarp0 * 32;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(q * 32) << 16);
+    float* box = reinterpret_cast<float*>(epi_smem + (warp - kXEpiWarp0) * 4096);
+    int buf = 0, parity = 0;
+    uint32_t tphase = 0;
+    bool alive = true;  // a wait that gave up: finish without waiting, so every barrier is met
+    for (int u = first; u < g.units; u += step) {
+        const XUnit w = x_unit(g, u);
+        const int i = w.tm * CG + static_cast<int>(rank);
+        const int i_in = min(i, g.mb - 1);
+        float acc[NB * 64];
+#pragma unroll
+        for (int j = 0; j < NB * 64; ++j) acc[j] = 0.0f;
+        for (int c = w.c0; c < w.c1; ++c) {
+            const int seg = EPI == kXF32 && c >= g.kc0 ? 1 : 0;
+            const int k = seg ? c - g.kc0 : c;
+            const float ia =
+                g.a[seg].inv[x_block(g.a[seg], w.z, i_in, k, x_flip(g.a[seg], w.tm * CG, k))];
+            float f1[NB], f2[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const XOperand& ob = EPI == kXGated ? g.b[b] : g.b[seg];
+                const int j0 = EPI == kXGated ? w.tn : w.tn * NB;
+                const int j = EPI == kXGated ? w.tn : min(j0 + b, g.nb - 1);
+                const float ib = ob.inv[x_block(ob, w.z, j, k, x_flip(ob, j0, k))];
+                f1[b] = fminf(ia, ib);  // smaller first: no overflow on the way
+                f2[b] = fmaxf(ia, ib);
+            }
+            if (alive) alive = mbar_wait(&tfull[buf], tphase, 1u << 2);
+            alive = __all_sync(0xffffffffu, alive);
+            tc_fence_after();
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    uint32_t r[16];
+                    tmem_ld_32x32b_x16(lanes + static_cast<uint32_t>(buf * NB * 128 + b * 128 +
+                                                                     half * 64 + t * 16), r);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        float& a = acc[b * 64 + t * 16 + j];
+                        a = fmaf(__uint_as_float(r[j]) * f1[b], f2[b], a);
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (CG == 1) {
+                    mbar_arrive(&tempty[buf]);
+                } else {
+                    mbar_arrive_cluster(mapa_shared(&tempty[buf], 0));
+                }
+            }
+            if (++buf == 2) {
+                buf = 0;
+                tphase ^= 1u;
+            }
+        }
+        if (g.splits > 1) {
+            // A split contraction: every part leaves its sums, and the part that finds itself
+            // counted last adds them in the parts' order (the same sum whichever that is).
+            constexpr int kPart = NB * 64 * kXEpiThreads;
+            float* mine = g.part + (static_cast<long long>(u) * CG + rank) * kPart;
+#pragma unroll
+            for (int j = 0; j < NB * 64; ++j) __stcg(mine + j * kXEpiThreads + et, acc[j]);
+            __threadfence();
+            epi_bar();
+            if (et == 0) {
+                int* n = g.count + w.tile * CG + rank;
+                const int before = atomicAdd(n, 1);
+                const int is_last = before == g.splits - 1 ? 1 : 0;
+                if (is_last) *n = 0;  // ready for the next launch
+                *last_flag = is_last;
+                __threadfence();
+            }
+            epi_bar();
+            const int is_last = *last_flag;
+            epi_bar();
+            if (!is_last) continue;
+#pragma unroll
+            for (int j = 0; j < NB * 64; ++j) acc[j] = 0.0f;
+            for (int s = 0; s < g.splits; ++s) {
+                const float* p =
+                    g.part +
+                    ((static_cast<long long>(w.tile) * g.splits + s) * CG + rank) * kPart;
+#pragma unroll
+                for (int j = 0; j < NB * 64; ++j) acc[j] += __ldcg(p + j * kXEpiThreads + et);
+            }
+        }
+        const bool row_block = i < g.mb;
+
+        if constexpr (EPI == kXF32 || EPI == kXSplit) {
+            // value = alpha acc + beta C
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const int jb = w.tn * NB + b;
+                if (g.beta != 0.0f && row_block && jb < g.nb) {
+                    const int blk = w.z * g.c.bstride + i * g.c.ldb + jb;
+                    const float f = g.c.inv[blk] * g.beta;
+                    const uint8_t* p = g.c.data + static_cast<long long>(blk) * kXBlockBytes +
+                                       half * 8 * kXLineBytes + row * 16;
+#pragma unroll
+                    for (int ch = 0; ch < 8; ++ch) {
+                        const uint4 hq = *reinterpret_cast<const uint4*>(p + ch * kXLineBytes);
+                        const uint4 lq = *reinterpret_cast<const uint4*>(p + ch * kXLineBytes +
+                                                                         kXBlockBytes / 2);
+                        const uint32_t hw[4] = {hq.x, hq.y, hq.z, hq.w};
+                        const uint32_t lw[4] = {lq.x, lq.y, lq.z, lq.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 hf =
+                                __half22float2(*reinterpret_cast<const __half2*>(&hw[e]));
+                            const float2 lf =
+                                __half22float2(*reinterpret_cast<const __half2*>(&lw[e]));
+                            float& a0 = acc[b * 64 + ch * 8 + e * 2];
+                            float& a1 = acc[b * 64 + ch * 8 + e * 2 + 1];
+                            a0 = fmaf(hf.x + lf.x, f, a0 * g.alpha);
+                            a1 = fmaf(hf.y + lf.y, f, a1 * g.alpha);
+                        }
+                    }
+                } else if (g.alpha != 1.0f) {
+#pragma unroll
+                    for (int j = 0; j < 64; ++j) acc[b * 64 + j] *= g.alpha;
+                }
+            }
+        }
+
+        if constexpr (EPI == kXF32) {
+            // through a 32 x 32 box (column c of row r at c ^ r: no bank conflicts), so that a
+            // warp writes 32 consecutive columns of one row at a time, whatever the row stride
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int col = (w.tn * NB + b) * kXBlk + half * 64 + t * 32 + lane;
+                    const int row0 = i * kXBlk + q * 32;
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        box[lane * 32 + (j ^ lane)] = acc[b * 64 + t * 32 + j];
+                    __syncwarp();
+                    if (row_block && col < g.n) {
+                        float* dst = g.out + w.z * g.out_bs +
+                                     static_cast<long long>(row0) * g.ld + col;
+                        const int rows = min(32, g.m - row0);
+#pragma unroll 8
+                        for (int r = 0; r < rows; ++r) {
+                            *dst = box[r * 32 + (lane ^ r)];
+                            dst += g.ld;
+                        }
+                    }
+                }
+            }
+        }
+
+        if constexpr (EPI == kXSplit) {
+            uint32_t* slot = red + parity * 4;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                float amax = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 64; ++j) amax = fmaxf(amax, finite_abs(acc[b * 64 + j]));
+                x_max_into(slot + b, amax);
+            }
+            parity = parity == 2 ? 0 : parity + 1;
+            if (et < 4) red[parity * 4 + et] = 0u;
+            epi_bar();
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const int jb = w.tn * NB + b;
+                if (row_block && jb < g.nb) {
+                    const int blk = w.z * g.o[0].bstride + i * g.o[0].ldb + jb;
+                    float s, inv;
+                    split_scale(__uint_as_float(slot[b]), s, inv);
+                    if (et == 0) g.o[0].inv[blk] = inv;
+                    uint8_t* dst = g.o[0].data + static_cast<long long>(blk) * kXBlockBytes;
+#pragma unroll
+                    for (int ch = 0; ch < 8; ++ch)
+                        store_split8(dst, half * 8 + ch, row, acc + b * 64 + ch * 8, s);
+                }
+            }
+        }
+
+        if constexpr (EPI == kXGated) {
+            // acc: 64 gate columns, then the same 64 up columns
+            uint32_t* slot = red + parity * 4;
+            const int blk = i_in * g.o[0].ldb + w.tn;
+            float gm = 0.0f, um = 0.0f, hm = 0.0f;
+            if (g.gate != nullptr) {
+#pragma unroll
+                for (int j = 0; j < 64; ++j) {
+                    gm = fmaxf(gm, finite_abs(acc[j]));
+                    um = fmaxf(um, finite_abs(acc[64 + j]));
+                }
+                if (row_block) {
+                    const long long at =
+                        (static_cast<long long>(blk) * 2 + half) * 64 * kXBlk + row * 4;
+#pragma unroll
+                    for (int j = 0; j < 64; j += 4) {
+                        *reinterpret_cast<float4*>(g.gate + at + j * kXBlk) =
+                            make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+                        *reinterpret_cast<float4*>(g.up + at + j * kXBlk) = make_float4(
+                            acc[64 + j], acc[64 + j + 1], acc[64 + j + 2], acc[64 + j + 3]);
+                    }
+                }
+                x_max_into(slot + 1, gm);
+                x_max_into(slot + 2, um);
+            }
+            if (g.store_h) {
+#pragma unroll
+                for (int j = 0; j < 64; ++j) {
+                    acc[j] = act_slope(acc[j], g.act).x * acc[64 + j];
+                    hm = fmaxf(hm, finite_abs(acc[j]));
+                }
+                x_max_into(slot, hm);
+            }
+            parity = parity == 2 ? 0 : parity + 1;
+            if (et < 4) red[parity * 4 + et] = 0u;
+            epi_bar();
+            if (row_block) {
+                if (g.gate != nullptr && et == 0) {
+                    g.gmax[blk * 2] = __uint_as_float(slot[1]);
+                    g.gmax[blk * 2 + 1] = __uint_as_float(slot[2]);
+                }
+                if (g.store_h) {
+                    float s, inv;
+                    split_scale(__uint_as_float(slot[0]), s, inv);
+                    if (et == 0) g.o[0].inv[blk] = inv;
+                    uint8_t* dst = g.o[0].data + static_cast<long long>(blk) * kXBlockBytes;
+#pragma unroll
+                    for (int ch = 0; ch < 8; ++ch)
+                        store_split8(dst, half * 8 + ch, row, acc + ch * 8, s);
+                }
+            }
+        }
+
+        if constexpr (EPI == kXGatedBwd) {
+            // acc: the gradient of h. The three outputs' scales come from bounds,
+            // |dgate| <= 1.13 max|dh| max|up|, |dup| <= max|dh| max|gate|,
+            // |h| <= max|gate| max|up|: a scale a few powers of two above the tightest one moves
+            // the range of a floating format, not its precision, and saves a pass.
+            uint32_t* slot = red + parity * 4;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                float amax = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 64; ++j) amax = fmaxf(amax, finite_abs(acc[b * 64 + j]));
+                x_max_into(slot + b, amax);
+            }
+            parity = parity == 2 ? 0 : parity + 1;
+            if (et < 4) red[parity * 4 + et] = 0u;
+            epi_bar();
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const int jb = w.tn * NB + b;
+                if (row_block && jb < g.nb) {
+                    const int blk = i * g.o[0].ldb + jb;
+                    const float dm = __uint_as_float(slot[b]);
+                    const float gm = g.gmax[blk * 2], um = g.gmax[blk * 2 + 1];
+                    float s0, s1, s2, i0, i1, i2;
+                    const float top = 3.402823466e38f;
+                    split_scale(fminf(dm * um * kXMaxSlope, top), s0, i0);
+                    split_scale(fminf(dm * gm, top), s1, i1);
+                    split_scale(fminf(gm * um, top), s2, i2);
+                    if (et == 0) {
+                        g.o[0].inv[blk] = i0;
+                        g.o[1].inv[blk] = i1;
+                        g.o[2].inv[blk] = i2;
+                    }
+                    const long long at =
+                        (static_cast<long long>(blk) * 2 + half) * 64 * kXBlk + row * 4;
+                    const long long off = static_cast<long long>(blk) * kXBlockBytes;
+#pragma unroll
+                    for (int ch = 0; ch < 8; ++ch) {
+                        float dg[8], du[8], hh[8];
+#pragma unroll
+                        for (int e = 0; e < 8; e += 4) {
+                            const float4 gv = *reinterpret_cast<const float4*>(
+                                g.gate + at + (ch * 8 + e) * kXBlk);
+                            const float4 uv = *reinterpret_cast<const float4*>(
+                                g.up + at + (ch * 8 + e) * kXBlk);
+                            const float gs[4] = {gv.x, gv.y, gv.z, gv.w};
+                            const float us[4] = {uv.x, uv.y, uv.z, uv.w};
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) {
+                                const float dh = acc[b * 64 + ch * 8 + e + x];
+                                const float2 as = act_slope(gs[x], g.act);
+                                dg[e + x] = dh * us[x] * as.y;
+                                du[e + x] = dh * as.x;
+                                hh[e + x] = as.x * us[x];
+                            }
+                        }
+                        store_split8(g.o[0].data + off, half * 8 + ch, row, dg, s0);
+                        store_split8(g.o[1].data + off, half * 8 + ch, row, du, s1);
+                        store_split8(g.o[2].data + off, half * 8 + ch, row, hh, s2);
+                    }
+                }
+            }
+        }
+    }
+}
+
+template <int CG, int NB, int EPI>
+__global__ void __launch_bounds__(kXThreads, 1)
+    split_mm_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mm,
+                    const __grid_constant__ XArgs g) {
+    using C = XConfig<CG, NB>;
+    extern __shared__ __align__(1024) uint8_t x_smem_raw[];
+    uint8_t* stages = reinterpret_cast<uint8_t*>(
+        (reinterpret_cast<uintptr_t>(x_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    uint8_t* epi_smem = stages + C::kStageArea;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(epi_smem + C::kEpiBytes);
+    uint64_t* full = bars;
+    uint64_t* empty = full + C::kStages;
+    uint64_t* tfull = empty + C::kStages;
+    uint64_t* tempty = tfull + 2;
+    uint64_t* drain = tempty + 2;
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain + 1);
+    uint32_t* red = tmem_holder + 1;                       // three sets of four block maxima
+    int* last_flag = reinterpret_cast<int*>(red + 12);
+
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t rank = CG == 1 ? 0u : cluster_ctarank();
+    const int first = static_cast<int>(blockIdx.x) / CG, step = static_cast<int>(gridDim.x) / CG;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&tfull[s], 1);
+            mbar_init(&tempty[s], 8 * CG);
+        }
+        mbar_init(drain, 1);
+        for (int s = 0; s < 12; ++s) red[s] = 0u;
+        fence_barrier_init();
+    }
+    if (warp == 0 && lane == 0) {
+        tma_prefetch_desc(&mk);
+        tma_prefetch_desc(&mm);
+    }
+    if (warp == 1) {
+        if constexpr (CG == 1) {
+            tmem_alloc(tmem_holder, C::kTmemCols);
+        } else {
+            tmem_alloc_cg2(tmem_holder, C::kTmemCols);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if constexpr (CG == 2) cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_holder;
+
+    if (warp == 0) {
+        if (lane == 0)
+            x_producer<CG, NB, EPI>(g, &mk, &mm, stages, full, empty, rank, first, step);
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            x_mma<CG, NB, EPI>(g, tmem, stages, full, empty, tfull, tempty, first, step);
+            // every MMA issued above must finish before TMEM is released, also on an error exit
+            if constexpr (CG == 1) {
+                mma_commit(drain);
+            } else {
+                mma_commit_cg2(drain);
+            }
+            mbar_wait(drain, 0, 1u << 1);
+        }
+        __syncwarp();
+    } else {
+        x_epilogue<CG, NB, EPI>(g, epi_smem, red, last_flag, tmem, tfull, tempty, rank, first,
+                                step);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if constexpr (CG == 2) cluster_sync();
+    if (warp == 1) {
+        tc_fence_after();
+        if constexpr (CG == 1) {
+            tmem_dealloc(tmem, C::kTmemCols);
+        } else {
+            tmem_dealloc_cg2(tmem, C::kTmemCols);
+        }
+    }
+}
+
+}  // namespace mfk
