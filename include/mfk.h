@@ -66,6 +66,7 @@ typedef enum mfk_precision {
 #define MFK_DEVERR_EPILOGUE_TIMEOUT 0x4u
 #define MFK_DEVERR_CONVERT_TIMEOUT 0x8u
 #define MFK_DEVERR_SELFTEST_TIMEOUT 0x10u
+#define MFK_DEVERR_INDEX 0x20u /* an embedding met an id outside its table */
 
 /* One GEMM: c = act(alpha * op(A) op(B) + beta * c_in + bias).
  * op(A) is m x k with element (i, p) at a[i*a_rs + p*a_cs]; op(B) is k x n with element (p, j)
@@ -407,6 +408,27 @@ int mfk_orthogonalize_f32(const float* update, int64_t batch, int64_t rows, int6
                           int64_t row_stride, int64_t batch_stride, float* out, int64_t ld,
                           int64_t out_batch_stride, int32_t steps, float a, float b, float c,
                           float eps, void* stream);
+
+/* The embedding lookup and the gradient of its table. ids: n whole numbers on the device, of
+ * id_bytes 4 or 8 (signed). No counterpart in the reference.
+ *
+ * mfk_embedding_f32: out[i] = scale * table[ids[i]] for the n ids; table is rows x d with row
+ * stride ld >= d, out n x d with row stride ld_out >= d. An id outside [0, rows) gives a row of
+ * zeros and sets MFK_DEVERR_INDEX in the device error word.
+ *
+ * mfk_embedding_grad_f32: out[v] = scale * (sum of grad[i] over the i with ids[i] == v) for every
+ * v of [0, rows): a dense gradient, rows that no id names are zeros. grad is n x d with row stride
+ * ld_grad >= d, out rows x d with row stride ld >= d (written, not added to). Tokens whose id is
+ * `padding` take no part (-1: none is left out); an id outside [0, rows) that is not `padding`
+ * takes no part either and sets MFK_DEVERR_INDEX. The sums are fp32, in an order that depends on
+ * the ids and sizes alone, so repeated calls give the same bits. The workspace (16 bytes per
+ * token, n d / 2 bytes at most for partial rows) comes from the stream-ordered allocator. */
+int mfk_embedding_f32(const float* table, int64_t rows, int64_t d, int64_t ld, const void* ids,
+                      int32_t id_bytes, int64_t n, float scale, float* out, int64_t ld_out,
+                      void* stream);
+int mfk_embedding_grad_f32(const float* grad, int64_t n, int64_t d, int64_t ld_grad,
+                           const void* ids, int32_t id_bytes, int64_t rows, float scale,
+                           int64_t padding, float* out, int64_t ld, void* stream);
 
 /* Process-wide precision used when a descriptor says MFK_PRECISION_DEFAULT. The reference's
  * public signatures have no precision argument, so its adapters leave the default in place. */

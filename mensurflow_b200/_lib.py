@@ -61,6 +61,8 @@ EXPORTED = (
     "mfk_gated_ffn_saved_floats",
     "mfk_gated_ffn_backward_f32",
     "mfk_orthogonalize_f32",
+    "mfk_embedding_f32",
+    "mfk_embedding_grad_f32",
     "mfk_set_default_precision",
     "mfk_get_default_precision",
     "mfk_device_status",
@@ -190,6 +192,9 @@ def lib() -> ctypes.CDLL:
                                                       ctypes.POINTER(GatedFfnGrads), vp, vp]
             so.mfk_orthogonalize_f32.argtypes = [vp, i64, i64, i64, i64, i64, vp, i64, i64, i32,
                                                  f32, f32, f32, f32, vp]
+            so.mfk_embedding_f32.argtypes = [vp, i64, i64, i64, vp, i32, i64, f32, vp, i64, vp]
+            so.mfk_embedding_grad_f32.argtypes = [vp, i64, i64, i64, vp, i32, i64, f32, i64, vp,
+                                                  i64, vp]
             so.mfk_set_default_precision.argtypes = [i32]
             so.mfk_get_default_precision.restype = i32
             so.mfk_device_status.argtypes = [ctypes.POINTER(ctypes.c_uint32), i32]

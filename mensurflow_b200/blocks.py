@@ -1,5 +1,5 @@
 """Operators of language models, on B200 tensors: the gated feed-forward block with its backward
-pass and the orthogonalised update, beside ``linear`` and ``linear_backward``.
+pass, the orthogonalised update and the embedding with its gradient, beside ``linear`` and ``linear_backward``.
 
 They follow the package's manner: fp32 CUDA tensors, work queued on the current stream of the
 tensors' device, explicit backward functions, ``ValueError`` for bad arguments and
@@ -220,4 +220,63 @@ def orthogonalize(update: torch.Tensor, steps: int = 5,
                                                u.stride(0) if batch > 1 else 0, out.data_ptr(),
                                                n, m * n, steps, a, b, c, float(eps), _stream()),
               op)
+    return out
+
+
+def _ids(op: str, ids: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
+    _require(ids, op, "ids")
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"{op}: ids must be int64 or int32, got {ids.dtype}")
+    if ids.device != like.device:
+        raise ValueError(f"{op}: tensors are on different devices; move one with Tensor::to()")
+    return ids.contiguous()
+
+
+def embedding(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """scale * table[ids]: the rows of ``table`` [rows, d] that ``ids`` (any shape, int64 or int32)
+    names, [*ids.shape, d]. An id outside the table gives a row of zeros and sets the bit
+    ``MFK_DEVERR_INDEX`` of ``device_status()``."""
+    op = "embedding"
+    _require(table, op, "table", 2)
+    index = _ids(op, ids, table)
+    _kernel_for(op, table)
+    rows, d = table.shape
+    if rows == 0 and index.numel() and d:
+        raise ValueError(f"{op}: the table has no rows")
+    with torch.cuda.device(table.device):
+        t = table if d <= 1 or table.stride(1) == 1 else contiguous(table)
+        out = torch.empty(tuple(ids.shape) + (d,), dtype=torch.float32, device=table.device)
+        check(_lib.lib().mfk_embedding_f32(_ptr(t), rows, d, max(t.stride(0), d), _ptr(index),
+                                           index.element_size(), index.numel(), float(scale),
+                                           _ptr(out), max(d, 1), _stream()), op)
+    return out
+
+
+def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, rows: int, scale: float = 1.0, *,
+                   padding: Optional[int] = None) -> torch.Tensor:
+    """The gradient of ``embedding``'s table, [rows, d]: scale times the sum of ``grad``
+    [*ids.shape, d] over the tokens of each id, zeros for ids that do not occur. Tokens of the id
+    ``padding`` take no part. Sums are fp32 over tokens sorted by id, in an order fixed by the ids:
+    repeated calls give the same bits. An id outside the table takes no part and sets
+    ``MFK_DEVERR_INDEX`` in ``device_status()``."""
+    op = "embedding_grad"
+    _require(grad, op, "grad", 1, at_least=True)
+    index = _ids(op, ids, grad)
+    if tuple(grad.shape[:-1]) != tuple(ids.shape):
+        raise ValueError(f"{op}: grad {tuple(grad.shape)} does not fit ids {tuple(ids.shape)}")
+    if not isinstance(rows, int) or rows < 0:
+        raise ValueError(f"{op}: rows must be a whole number of at least 0, got {rows!r}")
+    if padding is not None and not 0 <= padding < rows:
+        raise ValueError(f"{op}: padding {padding} is outside the table of {rows} rows")
+    _kernel_for(op, grad)
+    d, n = grad.shape[-1], index.numel()
+    with torch.cuda.device(grad.device):
+        g = _rows_of(grad, n, d)
+        if d > 1 and g.stride(1) != 1:
+            g = contiguous(g)
+        out = torch.empty((rows, d), dtype=torch.float32, device=grad.device)
+        check(_lib.lib().mfk_embedding_grad_f32(_ptr(g), n, d, g.stride(0) if n > 1 else max(d, 1),
+                                                _ptr(index), index.element_size(), rows,
+                                                float(scale), -1 if padding is None else padding,
+                                                _ptr(out), max(d, 1), _stream()), op)
     return out

@@ -1,0 +1,149 @@
+// Host side of the embedding kernels (embed.cuh). Part of the library's one translation unit.
+#pragma once
+
+namespace {
+
+int check_embed(int64_t rows, int64_t d, int64_t n, int32_t id_bytes) {
+    if (rows < 0 || d < 0 || n < 0 || (id_bytes != 4 && id_bytes != 8))
+        return MFK_ERR_INVALID_ARGUMENT;
+    if (rows > (int64_t(1) << 31) - 2 || n > (int64_t(1) << 31) - 4096 ||
+        d > (int64_t(1) << 31) - 4096)
+        return MFK_ERR_UNSUPPORTED;
+    return MFK_OK;
+}
+
+template <typename ID>
+int launch_embedding(const float* table, int64_t rows, int64_t d, int64_t ld, const ID* ids,
+                     int64_t n, float scale, float* out, int64_t ld_out, const DeviceInfo* info,
+                     cudaStream_t stream) {
+    const int vec = d % 4 == 0 && ld % 4 == 0 && ld_out % 4 == 0 && aligned16(table) &&
+                    aligned16(out);
+    const int64_t warps = n * ((d + 511) / 512);
+    const int64_t blocks = std::min<int64_t>((warps + 7) / 8, int64_t(info->sm_count) * 64);
+    mfk::embedding_kernel<ID><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
+        table, rows, static_cast<int>(d), ld, ids, n, scale, out, ld_out, vec);
+    g_launches.fetch_add(1);
+    MFK_CUDA(cudaGetLastError());
+    return MFK_OK;
+}
+
+int run_embedding_grad(const float* grad, int64_t n, int64_t d, int64_t ld_grad, const void* ids,
+                       int32_t id_bytes, int64_t rows, float scale, int64_t padding, float* out,
+                       int64_t ld, cudaStream_t stream) {
+    int rc = check_embed(rows, d, n, id_bytes);
+    if (rc != MFK_OK) return rc;
+    if (rows == 0 || d == 0) return MFK_OK;
+    if (out == nullptr || ld < d) return MFK_ERR_INVALID_ARGUMENT;
+    if (n > 0 && (grad == nullptr || ids == nullptr || (ld_grad < d && n > 1)))
+        return MFK_ERR_INVALID_ARGUMENT;
+    int dev = 0;
+    DeviceInfo* info = nullptr;
+    rc = current_device(&dev, &info);
+    if (rc != MFK_OK) return rc;
+    if (n == 0) return x_zero(out, rows, d, ld, stream);
+
+    const int vec = d % 4 == 0 && ld % 4 == 0 && ld_grad % 4 == 0 && aligned16(grad) &&
+                    aligned16(out);
+    const int pieces = static_cast<int>((d + mfk::kEmbedPiece - 1) / mfk::kEmbedPiece);
+    // windows: about eight blocks per SM, of 16 to 256 tokens
+    int window = 16;
+    while (window < mfk::kEmbedMaxWindow && n * pieces / (window * 2) >= info->sm_count * 8)
+        window *= 2;
+    const int64_t windows = (n + window - 1) / window;
+    const int tiles = static_cast<int>((n + mfk::kSortTile - 1) / mfk::kSortTile);
+    if (windows > (int64_t(1) << 31) - 1 || pieces > 65535) return MFK_ERR_UNSUPPORTED;
+
+    // one allocation: keys and positions twice, digit counts, the marks, the partial rows
+    const size_t items = (static_cast<size_t>(n) + 63) / 64 * 64;
+    const size_t counts = static_cast<size_t>(tiles) * 256;
+    const size_t marks = (static_cast<size_t>(rows) + 31) / 32 + 64;
+    const size_t part = static_cast<size_t>(windows) * 2 * static_cast<size_t>(d);
+    uint8_t* base = nullptr;
+    MFK_CUDA(cudaMallocAsync(reinterpret_cast<void**>(&base),
+                             (part + 4 * items + counts + marks + 64) * 4, stream));
+    struct Free {
+        void* p;
+        cudaStream_t s;
+        ~Free() { cudaFreeAsync(p, s); }
+    } release{base, stream};
+    float* d_part = reinterpret_cast<float*>(base);
+    uint32_t* words = reinterpret_cast<uint32_t*>(base) + (part + 63) / 64 * 64;
+    uint32_t* keys[2] = {words, words + items};
+    uint32_t* pos[2] = {words + 2 * items, words + 3 * items};
+    uint32_t* d_counts = words + 4 * items;
+    uint32_t* d_marks = d_counts + counts;
+    MFK_CUDA(cudaMemsetAsync(d_marks, 0, marks * 4, stream));
+
+    if (id_bytes == 8) {
+        mfk::embed_keys_kernel<int64_t><<<tiles, 256, 0, stream>>>(
+            static_cast<const int64_t*>(ids), n, rows, padding, keys[0], d_marks, d_counts, tiles);
+    } else {
+        mfk::embed_keys_kernel<int32_t><<<tiles, 256, 0, stream>>>(
+            static_cast<const int32_t*>(ids), n, rows, padding, keys[0], d_marks, d_counts, tiles);
+    }
+    g_launches.fetch_add(1);
+    const int64_t zero_blocks = std::min<int64_t>((rows + 7) / 8, int64_t(info->sm_count) * 64);
+    mfk::embed_zero_kernel<<<static_cast<unsigned>(zero_blocks), 256, 0, stream>>>(
+        d_marks, rows, static_cast<int>(d), out, ld, vec);
+    g_launches.fetch_add(1);
+    int at = 0;
+    for (int shift = 0; shift < 32 && (rows >> shift) != 0; shift += 8) {
+        if (shift > 0) {
+            mfk::sort_count_kernel<<<tiles, 256, 0, stream>>>(keys[at], n, shift, d_counts, tiles);
+            g_launches.fetch_add(1);
+        }
+        mfk::sort_scan_kernel<<<1, 1024, 0, stream>>>(d_counts, static_cast<int64_t>(counts));
+        mfk::sort_scatter_kernel<<<tiles, 256, 0, stream>>>(keys[at],
+                                                            shift > 0 ? pos[at] : nullptr, n, shift,
+                                                            d_counts, tiles, keys[at ^ 1],
+                                                            pos[at ^ 1]);
+        g_launches.fetch_add(2);
+        at ^= 1;
+    }
+    const dim3 grid(static_cast<unsigned>(windows), static_cast<unsigned>(pieces), 1);
+    mfk::embed_sum_kernel<<<grid, 256, 0, stream>>>(keys[at], pos[at], n, window,
+                                                    static_cast<uint32_t>(rows), grad, ld_grad,
+                                                    static_cast<int>(d), scale, out, ld, d_part,
+                                                    vec);
+    mfk::embed_join_kernel<<<grid, 256, 0, stream>>>(keys[at], n, window,
+                                                     static_cast<uint32_t>(rows),
+                                                     static_cast<int>(d), scale, out, ld, d_part,
+                                                     vec);
+    g_launches.fetch_add(2);
+    MFK_CUDA(cudaGetLastError());
+    return MFK_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mfk_embedding_f32(const float* table, int64_t rows, int64_t d, int64_t ld, const void* ids,
+                      int32_t id_bytes, int64_t n, float scale, float* out, int64_t ld_out,
+                      void* stream) {
+    int rc = check_embed(rows, d, n, id_bytes);
+    if (rc != MFK_OK) return rc;
+    if (n == 0 || d == 0) return MFK_OK;
+    if (rows == 0 || table == nullptr || ids == nullptr || out == nullptr || ld_out < d ||
+        (ld < d && rows > 1))
+        return MFK_ERR_INVALID_ARGUMENT;
+    int dev = 0;
+    DeviceInfo* info = nullptr;
+    rc = current_device(&dev, &info);
+    if (rc != MFK_OK) return rc;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (id_bytes == 8)
+        return launch_embedding(table, rows, d, ld, static_cast<const int64_t*>(ids), n, scale,
+                                out, ld_out, info, s);
+    return launch_embedding(table, rows, d, ld, static_cast<const int32_t*>(ids), n, scale, out,
+                            ld_out, info, s);
+}
+
+int mfk_embedding_grad_f32(const float* grad, int64_t n, int64_t d, int64_t ld_grad,
+                           const void* ids, int32_t id_bytes, int64_t rows, float scale,
+                           int64_t padding, float* out, int64_t ld, void* stream) {
+    return run_embedding_grad(grad, n, d, ld_grad, ids, id_bytes, rows, scale, padding, out, ld,
+                              static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -20,6 +20,7 @@
 
 #include "attn_tc.cuh"
 #include "blas1.cuh"
+#include "embed.cuh"
 #include "gemm_tc.cuh"
 #include "movement.cuh"
 #include "prep.cuh"
@@ -1566,6 +1567,7 @@ int mfk_copy_peer(void* dst, int32_t dst_device, const void* src, int32_t src_de
 }  // extern "C"
 
 #include "split_host.cuh"
+#include "embed_host.cuh"
 
 extern "C" {
 
@@ -1587,6 +1589,13 @@ int mfk_device_status(uint32_t* bits, int32_t clear) {
         const unsigned int zero = 0;
         MFK_CUDA(cudaMemcpyToSymbol(mfk::g_device_error, &zero, sizeof(zero)));
     }
+    unsigned int index = 0;
+    MFK_CUDA(cudaMemcpyFromSymbol(&index, mfk::g_index_error, sizeof(index)));
+    if (clear && index != 0) {
+        const unsigned int zero = 0;
+        MFK_CUDA(cudaMemcpyToSymbol(mfk::g_index_error, &zero, sizeof(zero)));
+    }
+    if (index != 0) v |= MFK_DEVERR_INDEX;
     *bits = v;
     return v != 0 ? MFK_ERR_DEVICE_FAULT : MFK_OK;
 }
