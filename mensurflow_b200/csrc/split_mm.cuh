@@ -28,6 +28,8 @@
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "mfk_ptx.cuh"
 
 namespace mfk {
@@ -39,6 +41,7 @@ constexpr int kXBlockLines = 32;
 constexpr int kXThreads = 320;             // TMA warp, MMA warp, eight epilogue warps
 constexpr int kXEpiWarp0 = 2;
 constexpr int kXEpiThreads = 256;
+constexpr int kXBoxFloats = 32 * 33;       // 32 x 32, rows one float apart from 32: no conflicts
 
 enum XEpi : int { kXF32 = 0, kXSplit = 1, kXGated = 2, kXGatedBwd = 3 };
 
@@ -121,22 +124,38 @@ __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64
 }
 
 // 32 lanes x 16 consecutive columns, landed when it returns.
-__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, float (&r)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
         "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
         "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-          "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]),
+          "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]),
+          "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
         : "r"(taddr)
         : "memory");
+}
+
+// a0 += r0 f, a1 += r1 f: one instruction for the pair.
+__device__ __forceinline__ void fma2(float& a0, float& a1, float r0, float r1, float f) {
+    asm("{\n\t.reg .b64 a, r, f;\n\t"
+        "mov.b64 a, {%0, %1};\n\t"
+        "mov.b64 r, {%2, %3};\n\t"
+        "mov.b64 f, {%4, %4};\n\t"
+        "fma.rn.f32x2 a, r, f, a;\n\t"
+        "mov.b64 {%0, %1}, a;\n\t}"
+        : "+f"(a0), "+f"(a1)
+        : "f"(r0), "f"(r1), "f"(f));
 }
 
 // kind::f16 with fp16 operands and an fp32 accumulator (fields as idesc_tf32; formats 0 = F16).
 __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool a_mn_major, bool b_mn_major) {
     return (1u << 4) | ((a_mn_major ? 1u : 0u) << 15) | ((b_mn_major ? 1u : 0u) << 16) |
            ((static_cast<uint32_t>(n) >> 3) << 17) | ((static_cast<uint32_t>(m) >> 4) << 24);
+}
+
+__device__ __forceinline__ void prefetch_l2(const void* p) {
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
 }
 
 __device__ __forceinline__ void epi_bar() {
@@ -159,13 +178,28 @@ __device__ __forceinline__ float finite_abs(float x) {
     return a <= 3.402823466e38f ? a : 0.0f;  // infinities and NaN do not set a block's scale
 }
 
-// (hi, lo) of two scaled values, packed. A non-finite value goes into hi alone.
-__device__ __forceinline__ void split_pair(float x0, float x1, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(x0, x1);
+// The largest finite |v[i]|: one instruction a value (a NaN is passed over), and only if an
+// infinity turns up a second look without them.
+template <int N>
+__device__ __forceinline__ float largest(const float* v) {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(v[i]));
+    if (m > 3.402823466e38f) {
+        m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) m = fmaxf(m, finite_abs(v[i]));
+    }
+    return m;
+}
+
+
+// (hi, lo) of s x0 and s x1, packed. A non-finite x makes lo NaN.
+__device__ __forceinline__ void split_pair(float x0, float x1, float s, uint32_t& hi,
+                                           uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x0 * s, x1 * s);
     const float2 hf = __half22float2(h);
-    const float l0 = fabsf(x0) <= 65504.0f ? x0 - hf.x : 0.0f;
-    const float l1 = fabsf(x1) <= 65504.0f ? x1 - hf.y : 0.0f;
-    const __half2 l = __floats2half2_rn(l0, l1);
+    const __half2 l = __floats2half2_rn(fmaf(x0, s, -hf.x), fmaf(x1, s, -hf.y));
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = *reinterpret_cast<const uint32_t*>(&l);
 }
@@ -174,10 +208,10 @@ __device__ __forceinline__ void split_pair(float x0, float x1, uint32_t& hi, uin
 __device__ __forceinline__ void store_split8(uint8_t* block, int chunk, int row, const float* v,
                                              float s) {
     uint4 h, l;
-    split_pair(v[0] * s, v[1] * s, h.x, l.x);
-    split_pair(v[2] * s, v[3] * s, h.y, l.y);
-    split_pair(v[4] * s, v[5] * s, h.z, l.z);
-    split_pair(v[6] * s, v[7] * s, h.w, l.w);
+    split_pair(v[0], v[1], s, h.x, l.x);
+    split_pair(v[2], v[3], s, h.y, l.y);
+    split_pair(v[4], v[5], s, h.z, l.z);
+    split_pair(v[6], v[7], s, h.w, l.w);
     uint8_t* p = block + chunk * kXLineBytes + row * 16;
     *reinterpret_cast<uint4*>(p) = h;
     *reinterpret_cast<uint4*>(p + kXBlockBytes / 2) = l;
@@ -248,14 +282,8 @@ __global__ void __launch_bounds__(256) split_blocks_kernel(const __grid_constant
             }
         }
     }
-    float amax = 0.0f;
+    const float amax = largest<64>(&v[0][0][0]);
     double sum = 0.0;
-#pragma unroll
-    for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) amax = fmaxf(amax, finite_abs(v[a][b][j]));
     if (t.sumsq != nullptr) {
 #pragma unroll
         for (int a = 0; a < 2; ++a)
@@ -324,26 +352,44 @@ __global__ void __launch_bounds__(256) split_normalize_kernel(const double* sums
 
 enum XAct : int { kXActNone = 0, kXActRelu = 1, kXActGelu = 2, kXActGeluTanh = 3, kXActSilu = 4 };
 
-// act(v) and act'(v) in fp32. silu and the tanh form of GELU go through the logistic function
-// s(z) = 1 / (1 + exp(-z)): 0.5 (1 + tanh z) = s(2 z).
-__device__ __forceinline__ float2 act_slope(float v, int act) {
-    if (act == kXActSilu) {
-        const float s = __frcp_rn(1.0f + expf(-v));
+// 1 / (1 + exp(-z)) to about 3 ulp; 0 where exp overflows.
+__device__ __forceinline__ float logistic(float z) { return __fdividef(1.0f, 1.0f + expf(-z)); }
+
+// act(v) and act'(v) in fp32. silu and the tanh form of GELU go through the logistic function s:
+// 0.5 (1 + tanh z) = s(2 z). The kind is a template parameter and the epilogues branch on it once
+// per tile: with the branch inside the unrolled loops the code of all kinds lies between one
+// element and the next, and fetching it took three quarters of the kernel's time.
+template <int ACT>
+__device__ __forceinline__ float2 act_slope(float v) {
+    if constexpr (ACT == kXActSilu) {
+        const float s = logistic(v);
         return make_float2(v * s, s * (1.0f + v * (1.0f - s)));
-    }
-    if (act == kXActRelu) return v > 0.0f ? make_float2(v, 1.0f) : make_float2(v == v ? 0.0f : v, 0.0f);
-    if (act == kXActGelu) {
+    } else if constexpr (ACT == kXActRelu) {
+        // NaN stays NaN
+        return v > 0.0f ? make_float2(v, 1.0f) : make_float2(v == v ? 0.0f : v, 0.0f);
+    } else if constexpr (ACT == kXActGelu) {
         const float phi = 0.5f * erfcf(v * -0.70710678118654752f);
         return make_float2(v * phi, phi + v * (0.39894228040143268f * expf(-0.5f * v * v)));
-    }
-    if (act == kXActGeluTanh) {
+    } else if constexpr (ACT == kXActGeluTanh) {
         const float w = fminf(fmaxf(v, -16.0f), 16.0f);  // the logistic is 0 or 1 beyond
-        const float z2 = 1.5957691216057308f * (w + 0.044715f * w * w * w);
-        const float s = __frcp_rn(1.0f + expf(-z2));
+        const float s = logistic(1.5957691216057308f * (w + 0.044715f * w * w * w));
         const float dz2 = 1.5957691216057308f * (1.0f + 0.134145f * w * w);
         return make_float2(v * s, s + w * s * (1.0f - s) * dz2);
+    } else {
+        return make_float2(v, 1.0f);
     }
-    return make_float2(v, 1.0f);
+}
+
+// Calls f with the activation as a compile-time constant.
+template <typename F>
+__device__ __forceinline__ void with_act(int act, F&& f) {
+    switch (act) {
+    case kXActSilu: f(std::integral_constant<int, kXActSilu>{}); break;
+    case kXActRelu: f(std::integral_constant<int, kXActRelu>{}); break;
+    case kXActGelu: f(std::integral_constant<int, kXActGelu>{}); break;
+    case kXActGeluTanh: f(std::integral_constant<int, kXActGeluTanh>{}); break;
+    default: f(std::integral_constant<int, kXActNone>{}); break;
+    }
 }
 
 // The largest |act'| over all inputs (GELU's is 1.1290): bounds the gate's gradient.
@@ -358,7 +404,7 @@ struct XConfig {
     static constexpr int kStages = kBBlocks == 2 ? 2 : 3;
     static constexpr int kTmemCols = NB * 256;          // two accumulators
     static constexpr int kStageArea = kStages * kStageBytes;
-    static constexpr int kEpiBytes = 8 * 4096;          // 32 x 32 floats per epilogue warp
+    static constexpr int kEpiBytes = 8 * kXBoxFloats * 4;  // one box per epilogue warp
     static constexpr int kSmemBytes = kStageArea + kEpiBytes + 1024 + 512;
 };
 
@@ -574,7 +620,7 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* epi_smem, ui
     const int row = q * 32 + lane;
     const int et = threadIdx.x - kXEpiWarp0 * 32;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(q * 32) << 16);
-    float* box = reinterpret_cast<float*>(epi_smem + (warp - kXEpiWarp0) * 4096);
+    float* box = reinterpret_cast<float*>(epi_smem) + (warp - kXEpiWarp0) * kXBoxFloats;
     int buf = 0, parity = 0;
     uint32_t tphase = 0;
     bool alive = true;  // a wait that gave up: finish without waiting, so every barrier is met
@@ -582,6 +628,19 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* epi_smem, ui
         const XUnit w = x_unit(g, u);
         const int i = w.tm * CG + static_cast<int>(rank);
         const int i_in = min(i, g.mb - 1);
+        if constexpr (EPI == kXGatedBwd) {
+            // the tile's gate and up into L2 while its product is computed
+            for (int b = 0; b < NB; ++b) {
+                const int jb = w.tn * NB + b;
+                if (i < g.mb && jb < g.nb && w.s == g.splits - 1) {
+                    const long long at = (static_cast<long long>(i) * g.o[0].ldb + jb) * 16384;
+                    for (int x = et * 32; x < 16384; x += kXEpiThreads * 32) {
+                        prefetch_l2(g.gate + at + x);
+                        prefetch_l2(g.up + at + x);
+                    }
+                }
+            }
+        }
         float acc[NB * 64];
 #pragma unroll
         for (int j = 0; j < NB * 64; ++j) acc[j] = 0.0f;
@@ -590,15 +649,18 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* epi_smem, ui
             const int k = seg ? c - g.kc0 : c;
             const float ia =
                 g.a[seg].inv[x_block(g.a[seg], w.z, i_in, k, x_flip(g.a[seg], w.tm * CG, k))];
-            float f1[NB], f2[NB];
+            float f1[NB], f2[NB];  // the two blocks' 1/s: multiplied together where that is safe
+            bool safe = true;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 const XOperand& ob = EPI == kXGated ? g.b[b] : g.b[seg];
                 const int j0 = EPI == kXGated ? w.tn : w.tn * NB;
                 const int j = EPI == kXGated ? w.tn : min(j0 + b, g.nb - 1);
                 const float ib = ob.inv[x_block(ob, w.z, j, k, x_flip(ob, j0, k))];
-                f1[b] = fminf(ia, ib);  // smaller first: no overflow on the way
+                f1[b] = fminf(ia, ib);  // else the smaller first: no overflow on the way
                 f2[b] = fmaxf(ia, ib);
+                const float f = ia * ib;
+                safe = safe && f > 1e-30f && f < 1e30f;
             }
             if (alive) alive = mbar_wait(&tfull[buf], tphase, 1u << 2);
             alive = __all_sync(0xffffffffu, alive);
@@ -607,13 +669,17 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* epi_smem, ui
             for (int b = 0; b < NB; ++b) {
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
-                    uint32_t r[16];
+                    float r[16];
                     tmem_ld_32x32b_x16(lanes + static_cast<uint32_t>(buf * NB * 128 + b * 128 +
                                                                      half * 64 + t * 16), r);
+                    float* a = acc + b * 64 + t * 16;
+                    if (safe) {
+                        const float f = f1[b] * f2[b];
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        float& a = acc[b * 64 + t * 16 + j];
-                        a = fmaf(__uint_as_float(r[j]) * f1[b], f2[b], a);
+                        for (int j = 0; j < 16; j += 2) fma2(a[j], a[j + 1], r[j], r[j + 1], f);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) a[j] = fmaf(r[j] * f1[b], f2[b], a[j]);
                     }
                 }
             }
@@ -701,8 +767,8 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* epi_smem, ui
         }
 
         if constexpr (EPI == kXF32) {
-            // through a 32 x 32 box (column c of row r at c ^ r: no bank conflicts), so that a
-            // warp writes 32 consecutive columns of one row at a time, whatever the row stride
+            // through a 32 x 32 box, so that a warp writes 32 consecutive columns of one row at a
+            // time, whatever the row stride
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
 #pragma unroll
@@ -712,7 +778,7 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* epi_smem, ui
                     __syncwarp();
 #pragma unroll
                     for (int j = 0; j < 32; ++j)
-                        box[lane * 32 + (j ^ lane)] = acc[b * 64 + t * 32 + j];
+                        box[lane * 33 + j] = acc[b * 64 + t * 32 + j];
                     __syncwarp();
                     if (row_block && col < g.n) {
                         float* dst = g.out + w.z * g.out_bs +
@@ -720,7 +786,7 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* epi_smem, ui
                         const int rows = min(32, g.m - row0);
 #pragma unroll 8
                         for (int r = 0; r < rows; ++r) {
-                            *dst = box[r * 32 + (lane ^ r)];
+                            *dst = box[r * 33 + lane];
                             dst += g.ld;
                         }
                     }
@@ -732,10 +798,7 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* epi_smem, ui
             uint32_t* slot = red + parity * 4;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                float amax = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 64; ++j) amax = fmaxf(amax, finite_abs(acc[b * 64 + j]));
-                x_max_into(slot + b, amax);
+                x_max_into(slot + b, largest<64>(acc + b * 64));
             }
             parity = parity == 2 ? 0 : parity + 1;
             if (et < 4) red[parity * 4 + et] = 0u;
@@ -760,13 +823,7 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* epi_smem, ui
             // acc: 64 gate columns, then the same 64 up columns
             uint32_t* slot = red + parity * 4;
             const int blk = i_in * g.o[0].ldb + w.tn;
-            float gm = 0.0f, um = 0.0f, hm = 0.0f;
             if (g.gate != nullptr) {
-#pragma unroll
-                for (int j = 0; j < 64; ++j) {
-                    gm = fmaxf(gm, finite_abs(acc[j]));
-                    um = fmaxf(um, finite_abs(acc[64 + j]));
-                }
                 if (row_block) {
                     const long long at =
                         (static_cast<long long>(blk) * 2 + half) * 64 * kXBlk + row * 4;
@@ -778,16 +835,17 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* epi_smem, ui
                             acc[64 + j], acc[64 + j + 1], acc[64 + j + 2], acc[64 + j + 3]);
                     }
                 }
-                x_max_into(slot + 1, gm);
-                x_max_into(slot + 2, um);
+                x_max_into(slot + 1, largest<64>(acc));
+                x_max_into(slot + 2, largest<64>(acc + 64));
             }
             if (g.store_h) {
+                with_act(g.act, [&](auto kind) {
 #pragma unroll
-                for (int j = 0; j < 64; ++j) {
-                    acc[j] = act_slope(acc[j], g.act).x * acc[64 + j];
-                    hm = fmaxf(hm, finite_abs(acc[j]));
-                }
-                x_max_into(slot, hm);
+                    for (int j = 0; j < 64; ++j) {
+                        acc[j] = act_slope<decltype(kind)::value>(acc[j]).x * acc[64 + j];
+                    }
+                });
+                x_max_into(slot, largest<64>(acc));
             }
             parity = parity == 2 ? 0 : parity + 1;
             if (et < 4) red[parity * 4 + et] = 0u;
@@ -817,10 +875,7 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* epi_smem, ui
             uint32_t* slot = red + parity * 4;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                float amax = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 64; ++j) amax = fmaxf(amax, finite_abs(acc[b * 64 + j]));
-                x_max_into(slot + b, amax);
+                x_max_into(slot + b, largest<64>(acc + b * 64));
             }
             parity = parity == 2 ? 0 : parity + 1;
             if (et < 4) red[parity * 4 + et] = 0u;
@@ -845,6 +900,7 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* epi_smem, ui
                     const long long at =
                         (static_cast<long long>(blk) * 2 + half) * 64 * kXBlk + row * 4;
                     const long long off = static_cast<long long>(blk) * kXBlockBytes;
+with_act(g.act, [&](auto kind) {
 #pragma unroll
                     for (int ch = 0; ch < 8; ++ch) {
                         float dg[8], du[8], hh[8];
@@ -859,7 +915,7 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* epi_smem, ui
 #pragma unroll
                             for (int x = 0; x < 4; ++x) {
                                 const float dh = acc[b * 64 + ch * 8 + e + x];
-                                const float2 as = act_slope(gs[x], g.act);
+                                const float2 as = act_slope<decltype(kind)::value>(gs[x]);
                                 dg[e + x] = dh * us[x] * as.y;
                                 du[e + x] = dh * as.x;
                                 hh[e + x] = as.x * us[x];
@@ -869,6 +925,7 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* epi_smem, ui
                         store_split8(g.o[1].data + off, half * 8 + ch, row, du, s1);
                         store_split8(g.o[2].data + off, half * 8 + ch, row, hh, s2);
                     }
+                    });
                 }
             }
         }
