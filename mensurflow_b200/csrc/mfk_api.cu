@@ -24,6 +24,7 @@
 #include "gemm_tc.cuh"
 #include "movement.cuh"
 #include "prep.cuh"
+#include "rows.cuh"
 #include "simt.cuh"
 #include "split_mm.cuh"
 

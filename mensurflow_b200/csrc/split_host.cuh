@@ -307,6 +307,12 @@ int x_zero(float* out, int64_t rows, int64_t cols, int64_t ld, cudaStream_t stre
     return MFK_OK;
 }
 
+}  // namespace
+
+#include "rows_host.cuh"
+
+namespace {
+
 // ---- the gated feed-forward block ------------------------------------------------------------
 
 constexpr int64_t kXMaxDim = (int64_t(1) << 31) - 256;
@@ -370,6 +376,8 @@ int run_gated_ffn(const mfk_gated_ffn_desc* d, float* y, int64_t ldy, float* sav
             MFK_CUDA(cudaMemsetAsync(saved, 0, gated_saved_floats(d->rows, d->f) * 4, stream));
         return x_zero(y, d->rows, d->d, ldy, stream);
     }
+    if (d->rows <= mfk::kRowsMax && saved == nullptr)
+        return run_gated_rows(d, y, ldy, ws.info, ws.dev, stream);
     mfk::XSources list{};
     XMat x, wg, wu, wd;
     if (!x_source(ws, list, &x, d->x, d->rows, d->d, d->x_rs, d->x_cs) ||
