@@ -17,10 +17,23 @@ import torch
 
 from . import _lib
 from ._lib import GatedFfnDesc, GatedFfnGrads, check
-from .ops import _kernel_for, _require, _same, _stream, contiguous
+from .ops import _kernel_for, _require, _same, contiguous
 
 _GATED_ACTS = {None: _lib.ACT_NONE, "none": _lib.ACT_NONE, "relu": _lib.ACT_RELU,
                "gelu": _lib.ACT_GELU, "gelu_tanh": _lib.ACT_GELU_TANH, "silu": _lib.ACT_SILU}
+
+
+def _run(device: torch.device, op: str, call, *args) -> None:
+    """call(*args, stream) with the current stream of `device`, which is made current first. These
+    operators run for a few microseconds at their smallest, so the usual case costs no context
+    manager and no Stream object."""
+    if torch.cuda.current_device() == device.index:
+        status = call(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with torch.cuda.device(device):
+            status = call(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if status:
+        check(status, op)
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -57,7 +70,31 @@ class GatedSaved:
         self.features = features
 
 
+def _gated_fast(x, w_gate, w_up, w_down, activation, transpose_w):
+    """The descriptor of a call whose tensors are all contiguous fp32 matrices of one device that
+    fit each other; None for any other call, which `_gated_args` checks and lays out."""
+    try:
+        rows, d = x.shape
+        f = w_gate.shape[0 if transpose_w else 1]
+        inner, outer = ((f, d), (d, f)) if transpose_w else ((d, f), (f, d))
+        if not (x.is_cuda and rows > 0 and d > 1 and f > 1 and w_gate.shape == inner and
+                w_up.shape == inner and w_down.shape == outer):
+            return None
+        device = x.device
+        for t in (x, w_gate, w_up, w_down):
+            if t.dtype is not torch.float32 or not t.is_contiguous() or t.device != device:
+                return None
+        ws, ds = ((1, d), (1, f)) if transpose_w else ((f, 1), (d, 1))
+        return GatedFfnDesc(x.data_ptr(), d, 1, w_gate.data_ptr(), *ws, w_up.data_ptr(), *ws,
+                            w_down.data_ptr(), *ds, rows, d, f, _GATED_ACTS[activation], 0)
+    except (AttributeError, IndexError, KeyError, TypeError, ValueError):
+        return None
+
+
 def _gated_args(op, x, w_gate, w_up, w_down, activation, transpose_w):
+    desc = _gated_fast(x, w_gate, w_up, w_down, activation, transpose_w)
+    if desc is not None:
+        return desc, (x, w_gate, w_up, w_down)
     _require(x, op, "x", 1, at_least=True)
     for t, name in ((w_gate, "w_gate"), (w_up, "w_up"), (w_down, "w_down")):
         _require(t, op, name, 2)
@@ -124,15 +161,13 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     give non-finite results, though an infinity may come out as NaN."""
     desc, keep = _gated_args("gated_ffn", x, w_gate, w_up, w_down, activation, transpose_w)
     rows, d, f = desc.rows, desc.d, desc.f
-    with torch.cuda.device(x.device):
-        y = torch.empty(tuple(x.shape), dtype=torch.float32, device=x.device)
-        saved = None
-        if save:
-            size = _lib.lib().mfk_gated_ffn_saved_floats(rows, f)
-            saved = GatedSaved(torch.empty(size, dtype=torch.float32, device=x.device), rows, f)
-        check(_lib.lib().mfk_gated_ffn_f32(ctypes.byref(desc), _ptr(y), max(d, 1),
-                                           _ptr(saved.buffer) if save else None, _stream()),
-              "gated_ffn")
+    so = _lib.lib()
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    saved = None
+    if save:
+        saved = GatedSaved(x.new_empty(so.mfk_gated_ffn_saved_floats(rows, f)), rows, f)
+    _run(x.device, "gated_ffn", so.mfk_gated_ffn_f32, ctypes.byref(desc), _ptr(y), d or 1,
+         _ptr(saved.buffer) if save else None)
     return (y, saved) if save else y
 
 
@@ -159,25 +194,22 @@ def gated_ffn_backward(grad: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor
                              f"{saved.features} features)")
     if not need_x and not need_w:
         return None, None, None, None
-    with torch.cuda.device(x.device):
-        g2 = _rows_of(grad, rows, d)
-        o = GatedFfnGrads()
-        o.grad = _ptr(g2)
-        o.grad_rs, o.grad_cs = _strides(g2)
-        dx = dw_gate = dw_up = dw_down = None
-        if need_x:
-            dx = torch.empty(tuple(x.shape), dtype=torch.float32, device=x.device)
-            o.dx, o.ld_dx = _ptr(dx), max(d, 1)
-        if need_w:
-            dw_gate, dw_up, dw_down = (torch.empty(tuple(t.shape), dtype=torch.float32,
-                                                   device=x.device)
-                                       for t in (w_gate, w_up, w_down))
-            o.dw_gate, o.dw_up, o.dw_down = _ptr(dw_gate), _ptr(dw_up), _ptr(dw_down)
-            o.dw_rs, o.dw_cs = (1, max(d, 1)) if transpose_w else (max(f, 1), 1)
-            o.dw_down_rs, o.dw_down_cs = (1, max(f, 1)) if transpose_w else (max(d, 1), 1)
-        check(_lib.lib().mfk_gated_ffn_backward_f32(
-            ctypes.byref(desc), ctypes.byref(o), _ptr(saved.buffer) if saved else None,
-            _stream()), op)
+    g2 = _rows_of(grad, rows, d)
+    o = GatedFfnGrads()
+    o.grad = _ptr(g2)
+    o.grad_rs, o.grad_cs = _strides(g2)
+    dx = dw_gate = dw_up = dw_down = None
+    if need_x:
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+        o.dx, o.ld_dx = _ptr(dx), max(d, 1)
+    if need_w:
+        dw_gate, dw_up, dw_down = (torch.empty_like(t, memory_format=torch.contiguous_format)
+                                   for t in (w_gate, w_up, w_down))
+        o.dw_gate, o.dw_up, o.dw_down = _ptr(dw_gate), _ptr(dw_up), _ptr(dw_down)
+        o.dw_rs, o.dw_cs = (1, max(d, 1)) if transpose_w else (max(f, 1), 1)
+        o.dw_down_rs, o.dw_down_cs = (1, max(f, 1)) if transpose_w else (max(d, 1), 1)
+    _run(x.device, op, _lib.lib().mfk_gated_ffn_backward_f32, ctypes.byref(desc),
+         ctypes.byref(o), _ptr(saved.buffer) if saved else None)
     return dx, dw_gate, dw_up, dw_down
 
 
@@ -200,26 +232,23 @@ def orthogonalize(update: torch.Tensor, steps: int = 5,
     _kernel_for(op, update)
     m, n = update.shape[-2:]
     if update.numel() == 0:
-        return torch.empty(tuple(update.shape), dtype=torch.float32, device=update.device)
-    with torch.cuda.device(update.device):
-        if update.stride(-1) != 1 and n > 1 and (update.stride(-2) == 1 or m <= 1):
-            return orthogonalize(update.transpose(-2, -1), steps, coefficients,
-                                 eps).transpose(-2, -1)
-        u = update
-        if n > 1 and u.stride(-1) != 1:
-            u = contiguous(u)
-        try:
-            u = u.view(-1, m, n)
-        except RuntimeError:
-            u = contiguous(u).view(-1, m, n)
-        out = torch.empty(tuple(update.shape), dtype=torch.float32, device=update.device)
-        batch = u.shape[0]
-        a, b, c = (float(v) for v in coefficients)
-        check(_lib.lib().mfk_orthogonalize_f32(u.data_ptr(), batch, m, n,
-                                               u.stride(1) if m > 1 else n,
-                                               u.stride(0) if batch > 1 else 0, out.data_ptr(),
-                                               n, m * n, steps, a, b, c, float(eps), _stream()),
-              op)
+        return torch.empty_like(update, memory_format=torch.contiguous_format)
+    if n > 1 and update.stride(-1) != 1 and (update.stride(-2) == 1 or m <= 1):
+        return orthogonalize(update.transpose(-2, -1), steps, coefficients,
+                             eps).transpose(-2, -1)
+    u = update
+    if n > 1 and u.stride(-1) != 1:
+        u = contiguous(u)
+    try:
+        u = u.view(-1, m, n)
+    except RuntimeError:
+        u = contiguous(u).view(-1, m, n)
+    out = torch.empty_like(update, memory_format=torch.contiguous_format)
+    batch = u.shape[0]
+    a, b, c = (float(v) for v in coefficients)
+    _run(update.device, op, _lib.lib().mfk_orthogonalize_f32, u.data_ptr(), batch, m, n,
+         u.stride(1) if m > 1 else n, u.stride(0) if batch > 1 else 0, out.data_ptr(), n, m * n,
+         steps, a, b, c, float(eps))
     return out
 
 
@@ -241,14 +270,15 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0) -> tor
     index = _ids(op, ids, table)
     _kernel_for(op, table)
     rows, d = table.shape
-    if rows == 0 and index.numel() and d:
+    n = index.numel()
+    if rows == 0 and n and d:
         raise ValueError(f"{op}: the table has no rows")
-    with torch.cuda.device(table.device):
-        t = table if d <= 1 or table.stride(1) == 1 else contiguous(table)
-        out = torch.empty(tuple(ids.shape) + (d,), dtype=torch.float32, device=table.device)
-        check(_lib.lib().mfk_embedding_f32(_ptr(t), rows, d, max(t.stride(0), d), _ptr(index),
-                                           index.element_size(), index.numel(), float(scale),
-                                           _ptr(out), max(d, 1), _stream()), op)
+    t = table if d <= 1 or table.stride(1) == 1 else contiguous(table)
+    out = table.new_empty(ids.shape + (d,))
+    if n and d:
+        _run(table.device, op, _lib.lib().mfk_embedding_f32, t.data_ptr(), rows, d,
+             max(t.stride(0), d), index.data_ptr(), index.element_size(), n, float(scale),
+             out.data_ptr(), d)
     return out
 
 
@@ -264,19 +294,17 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, rows: int, scale: floa
     index = _ids(op, ids, grad)
     if tuple(grad.shape[:-1]) != tuple(ids.shape):
         raise ValueError(f"{op}: grad {tuple(grad.shape)} does not fit ids {tuple(ids.shape)}")
-    if not isinstance(rows, int) or rows < 0:
+    if not isinstance(rows, int) or isinstance(rows, bool) or rows < 0:
         raise ValueError(f"{op}: rows must be a whole number of at least 0, got {rows!r}")
     if padding is not None and not 0 <= padding < rows:
         raise ValueError(f"{op}: padding {padding} is outside the table of {rows} rows")
     _kernel_for(op, grad)
     d, n = grad.shape[-1], index.numel()
-    with torch.cuda.device(grad.device):
-        g = _rows_of(grad, n, d)
-        if d > 1 and g.stride(1) != 1:
-            g = contiguous(g)
-        out = torch.empty((rows, d), dtype=torch.float32, device=grad.device)
-        check(_lib.lib().mfk_embedding_grad_f32(_ptr(g), n, d, g.stride(0) if n > 1 else max(d, 1),
-                                                _ptr(index), index.element_size(), rows,
-                                                float(scale), -1 if padding is None else padding,
-                                                _ptr(out), max(d, 1), _stream()), op)
+    g = _rows_of(grad, n, d)
+    if d > 1 and g.stride(1) != 1:
+        g = contiguous(g)
+    out = grad.new_empty((rows, d))
+    _run(grad.device, op, _lib.lib().mfk_embedding_grad_f32, _ptr(g), n, d,
+         g.stride(0) if n > 1 else max(d, 1), _ptr(index), index.element_size(), rows,
+         float(scale), -1 if padding is None else padding, _ptr(out), max(d, 1))
     return out

@@ -4,31 +4,45 @@
 namespace {
 
 // One product of few rows: picks the kernel by the weights' orientation and alignment, the tile
-// width and the depth's shares (a cluster of 1 to 8 CTAs) so that about three CTAs per SM run.
+// width and the depth's shares (a cluster of 1 to 8 CTAs).
 struct RowsLaunch {
     cudaStream_t stream;
     const DeviceInfo* info;
     int device;
     bool dependent;  // may start while the launch before still runs
 
+    // Bytes on the longest path of a launch of `tiles` x ranks CTAs, two per SM: whole waves of
+    // a share of the depth, plus about 4 us of start and finish a wave (90 KB at a CTA's share of
+    // HBM). Fewer, longer waves beat an even number of shares: 8 rows, 4096 x 11008, gate and up
+    // in 86 tiles: 106 us as 8 shares (2.3 waves), 80 us as 3 (0.9 waves).
+    int64_t cost(int64_t tiles, int64_t depth, int64_t row_bytes, int* ranks) const {
+        int64_t best = 0;
+        *ranks = 1;
+        for (int r = 1; r <= mfk::kRowsRanks && (r == 1 || depth >= r * 32); ++r) {
+            const int64_t slots = int64_t(info->sm_count) * 2;
+            const int64_t waves = (tiles * r + slots - 1) / slots;
+            const int64_t c = waves * ((depth + r - 1) / r * row_bytes + 90000);
+            if (best == 0 || c < best) {
+                best = c;
+                *ranks = r;
+            }
+        }
+        return best;
+    }
+
     template <void (*kernel)(mfk::RowsArgs)>
-    int go(const mfk::RowsArgs& g, int64_t tiles, int64_t depth_per_share) const {
-        int ranks = 1;
-        while (ranks < 8 && tiles * ranks < int64_t(info->sm_count) * 3 &&
-               g.depth >= depth_per_share * ranks * 2)
-            ranks *= 2;
-        constexpr int kSmem = mfk::kRowsXBytes + mfk::kRowsRedBytes;
+    int go(const mfk::RowsArgs& g, int64_t tiles, int ranks) const {
         static std::atomic<uint64_t> ready{0};  // a bit per device
         if ((ready.load() >> device & 1u) == 0u) {
             MFK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                          kSmem));
+                                          mfk::kRowsSmem));
             ready.fetch_or(uint64_t(1) << device);
         }
         cudaLaunchConfig_t cfg = {};
         cudaLaunchAttribute attr[2];
         cfg.gridDim = dim3(static_cast<unsigned>(tiles * ranks), 1, 1);
         cfg.blockDim = dim3(256, 1, 1);
-        cfg.dynamicSmemBytes = kSmem;
+        cfg.dynamicSmemBytes = mfk::kRowsSmem;
         cfg.stream = stream;
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim.x = static_cast<unsigned>(ranks);
@@ -50,21 +64,29 @@ struct RowsLaunch {
     int run(const mfk::RowsArgs& g, bool depth_contiguous) const {
         const bool same4 = aligned16(g.w0) && g.ld0 % 4 == 0 &&
                            (W == 1 || (aligned16(g.w1) && g.ld1 % 4 == 0));
+        int ranks = 1;
         if (depth_contiguous) {
             const int64_t tiles = (g.cols + 15) / 16;
+            cost(tiles, g.depth, 64 * W, &ranks);
             if (same4 && g.depth % 4 == 0)
-                return go<mfk::rows_k_kernel<MT, 4, W>>(g, tiles, 256);
-            return go<mfk::rows_k_kernel<MT, 1, W>>(g, tiles, 256);
+                return go<mfk::rows_k_kernel<MT, 4, W>>(g, tiles, ranks);
+            return go<mfk::rows_k_kernel<MT, 1, W>>(g, tiles, ranks);
         }
-        // wide tiles where they still give two CTAs per SM with the depth in eight shares
-        const int64_t want = int64_t(info->sm_count) * 2;
-        if constexpr (MT <= 8) {
-            if (same4 && g.cols % 4 == 0 && (g.cols + 127) / 128 * 8 >= want)
-                return go<mfk::rows_n_kernel<MT, 4, W>>(g, (g.cols + 127) / 128, 64);
+        // tiles of 128, 64 or 32 columns by that cost, narrow ones a little dearer per byte
+        const int64_t t4 = (g.cols + 127) / 128, t2 = (g.cols + 63) / 64, t1 = (g.cols + 31) / 32;
+        int r4 = 1, r2 = 1, r1 = 1;
+        const double c4 = static_cast<double>(cost(t4, g.depth, 512 * W, &r4));
+        const double c2 = 1.1 * static_cast<double>(cost(t2, g.depth, 256 * W, &r2));
+        const double c1 = 1.3 * static_cast<double>(cost(t1, g.depth, 128 * W, &r1));
+        constexpr bool kWide = MT * W <= 16;  // 64 sums a lane at most
+        const bool can4 = kWide && same4 && g.cols % 4 == 0;
+        const bool can2 = same4 && g.cols % 2 == 0;
+        if constexpr (kWide) {
+            if (can4 && c4 <= c2 && c4 <= c1)
+                return go<mfk::rows_n_kernel<MT, 4, W>>(g, t4, r4);
         }
-        if (same4 && g.cols % 2 == 0 && (g.cols + 63) / 64 * 8 >= want)
-            return go<mfk::rows_n_kernel<MT, 2, W>>(g, (g.cols + 63) / 64, 64);
-        return go<mfk::rows_n_kernel<MT, 1, W>>(g, (g.cols + 31) / 32, 64);
+        if (can2 && c2 <= c1) return go<mfk::rows_n_kernel<MT, 2, W>>(g, t2, r2);
+        return go<mfk::rows_n_kernel<MT, 1, W>>(g, t1, r1);
     }
 
     template <int W>
