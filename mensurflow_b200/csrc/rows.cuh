@@ -160,7 +160,8 @@ __global__ void __launch_bounds__(256, 2) rows_n_kernel(RowsArgs g) {
     constexpr int kStages = 8;
     constexpr int kDup = VEC == 1 ? 1 : 2;
     constexpr int kTurn = 8 * kR;                        // depth of a turn of the eight warps
-    constexpr int kXTurns = kRowsXBytes / 4 / kDup / MT / kTurn;
+    constexpr int kXTurns = kRowsXBytes / 4 / kDup / MT / kTurn / kStages * kStages;
+    static_assert(kXTurns > 0, "the ring turns within the staged x");
     extern __shared__ __align__(16) float rows_smem[];
     float* xs = rows_smem;                               // [depth][MT][kDup]
     float* red = rows_smem + kRowsXBytes / 4;
@@ -187,17 +188,23 @@ __global__ void __launch_bounds__(256, 2) rows_n_kernel(RowsArgs g) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) acc[i][r][e] = 0.0f;
 
-    auto issue = [&](int turn) {
-        if (turn < turns) {
+    // the next turn's rows: running pointers, this warp's first row of the turn
+    const float* q0 = p0 + static_cast<long long>(k_begin + warp * kR) * g.ld0;
+    const float* q1 = W == 2 ? p1 + static_cast<long long>(k_begin + warp * kR) * g.ld1 : nullptr;
+    const long long step0 = g.ld0 * kTurn, step1 = W == 2 ? g.ld1 * kTurn : 0;
+    int next = warp * kR;
+    auto issue = [&](int stage) {
 #pragma unroll
-            for (int j = 0; j < kR; ++j) {
-                // rows past the end repeat the last one and are not used
-                const long long row = k_begin + min((turn * 8 + warp) * kR + j, depth - 1);
-                float* dst = ring + (turn % kStages) * 256 + j * W * kTile;
-                rows_copy<VEC * 4>(dst, p0 + row * g.ld0);
-                if constexpr (W == 2) rows_copy<VEC * 4>(dst + kTile, p1 + row * g.ld1);
+        for (int j = 0; j < kR; ++j) {
+            if (next + j < depth) {
+                float* dst = ring + stage * 256 + j * W * kTile;
+                rows_copy<VEC * 4>(dst, q0 + j * g.ld0);
+                if constexpr (W == 2) rows_copy<VEC * 4>(dst + kTile, q1 + j * g.ld1);
             }
         }
+        q0 += step0;
+        if constexpr (W == 2) q1 += step1;
+        next += kTurn;
         cp_async_commit();
     };
     for (int t = 0; t < kStages; ++t) issue(t);   // on the way while x is staged
@@ -209,39 +216,47 @@ __global__ void __launch_bounds__(256, 2) rows_n_kernel(RowsArgs g) {
                                MT * kDup);
         __syncthreads();
         const int t1 = min(turns, t0 + kXTurns);
-        for (int t = t0; t < t1; ++t) {
-            cp_async_wait<kStages - 1>();
+        const float* xr = xs + warp * kR * (MT * kDup);
+        int left = depth - x0 - warp * kR;               // rows of the depth from this warp's first
+        for (int t = t0; t < t1; t += kStages) {
 #pragma unroll
-            for (int j = 0; j < kR; ++j) {
-                const int k = (t * 8 + warp) * kR + j;
-                if (k < depth) {
-                    float w[W][VEC];
-                    const float* src = ring + (t % kStages) * 256 + j * W * kTile;
+            for (int u = 0; u < kStages; ++u) {
+                if (t + u < t1) {
+                    cp_async_wait<kStages - 1>();
 #pragma unroll
-                    for (int i = 0; i < W; ++i) rows_read<VEC>(src + i * kTile, w[i]);
-                    const float* xr = xs + (k - x0) * (MT * kDup);
-                    if constexpr (VEC == 1) {
+                    for (int j = 0; j < kR; ++j) {
+                        if (j < left) {
+                            float w[W][VEC];
+                            const float* src = ring + u * 256 + j * W * kTile;
 #pragma unroll
-                        for (int r = 0; r < MT; ++r)
+                            for (int i = 0; i < W; ++i) rows_read<VEC>(src + i * kTile, w[i]);
+                            const float* xj = xr + j * (MT * kDup);
+                            if constexpr (VEC == 1) {
 #pragma unroll
-                            for (int i = 0; i < W; ++i)
-                                acc[i][r][0] = fmaf(xr[r], w[i][0], acc[i][r][0]);
-                    } else {
+                                for (int r = 0; r < MT; ++r)
 #pragma unroll
-                        for (int r = 0; r < MT; ++r) {
-                            const unsigned long long xv =
-                                reinterpret_cast<const unsigned long long*>(xr)[r];
+                                    for (int i = 0; i < W; ++i)
+                                        acc[i][r][0] = fmaf(xj[r], w[i][0], acc[i][r][0]);
+                            } else {
 #pragma unroll
-                            for (int i = 0; i < W; ++i)
+                                for (int r = 0; r < MT; ++r) {
+                                    const unsigned long long xv =
+                                        reinterpret_cast<const unsigned long long*>(xj)[r];
 #pragma unroll
-                                for (int e = 0; e < VEC; e += 2)
-                                    fma2_pair(acc[i][r][e], acc[i][r][e + 1], w[i][e],
-                                              w[i][e + 1], xv);
+                                    for (int i = 0; i < W; ++i)
+#pragma unroll
+                                        for (int e = 0; e < VEC; e += 2)
+                                            fma2_pair(acc[i][r][e], acc[i][r][e + 1], w[i][e],
+                                                      w[i][e + 1], xv);
+                                }
+                            }
                         }
                     }
+                    issue(u);
+                    xr += kTurn * MT * kDup;
+                    left -= kTurn;
                 }
             }
-            issue(t + kStages);
         }
     }
     cp_async_wait<0>();
