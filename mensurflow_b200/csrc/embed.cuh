@@ -207,25 +207,152 @@ __global__ void __launch_bounds__(256)
     }
 }
 
-// ---- the sums --------------------------------------------------------------------------------
+// ---- the sort in one launch ------------------------------------------------------------------
 
-// Zeros in the rows that no token names: one warp per row.
-__global__ void __launch_bounds__(256)
-    embed_zero_kernel(const uint32_t* __restrict__ present, long long rows, int d,
-                      float* __restrict__ out, long long ld, int vec) {
-    const int lane = threadIdx.x & 31;
-    for (long long v = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) >> 5; v < rows;
-         v += static_cast<long long>(gridDim.x) * 8) {
-        if ((present[v >> 5] >> (v & 31)) & 1u) continue;
-        float* p = out + v * ld;
-        if (vec) {
-            for (int c = lane * 4; c < d; c += 128)
-                *reinterpret_cast<float4*>(p + c) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        } else {
-            for (int c = lane; c < d; c += 32) p[c] = 0.0f;
+constexpr int kClusterSortRanks = 8;
+constexpr int kClusterSortMax = kClusterSortRanks * 8192;   // tokens
+
+__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+// Up to 65536 tokens in one cluster of up to 8 CTAs: each holds `chunk` of the list in shared
+// memory and a pass scatters straight into the others'. Ranks within a warp's items as in
+// sort_scatter_kernel, then over the CTA's warps, then over the CTAs. Also clears the marks and
+// sets those of the ids that are present. IT: rounds of 32 items per warp.
+template <typename ID, int IT>
+__global__ void __launch_bounds__(1024, 1)
+    embed_sort_kernel(const ID* __restrict__ ids, int n, int chunk, long long rows,
+                      long long padding, int passes, uint32_t* __restrict__ present,
+                      uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out) {
+    extern __shared__ __align__(16) uint32_t sort_smem[];
+    uint32_t* buffers = sort_smem;                         // keys, positions; twice
+    uint32_t* counts = sort_smem + 4 * chunk;              // [32 warps][256]
+    uint32_t* total = counts + 32 * 256;                   // [256] this CTA's
+    uint32_t* base = total + 256;                          // [256]
+    uint32_t* scan = base + 256;                           // [8]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int ranks = static_cast<int>(gridDim.x);         // one cluster
+    const int rank = static_cast<int>(cluster_ctarank());
+    const int first = rank * chunk;
+    const int count = max(0, min(chunk, n - first));
+
+    const long long words = (rows + 31) / 32;
+    for (long long i = rank * 1024 + static_cast<int>(threadIdx.x); i < words; i += ranks * 1024)
+        present[i] = 0u;
+    __threadfence();
+    cluster_sync();
+
+    const int mine = warp * IT * 32 + lane;                // first item of this lane
+    uint32_t key[IT], pos[IT];
+#pragma unroll
+    for (int r = 0; r < IT; ++r) {
+        const int i = mine + r * 32;
+        key[r] = 0u;
+        pos[r] = static_cast<uint32_t>(first + i);
+        if (i < count) {
+            const long long id = static_cast<long long>(ids[first + i]);
+            const bool inside = id >= 0 && id < rows;
+            if (!inside && id != padding) atomicOr(&g_index_error, 1u);
+            key[r] = static_cast<uint32_t>(inside && id != padding ? id : rows);
+            if (key[r] < rows) {
+                uint32_t* word = present + (key[r] >> 5);
+                const uint32_t bit = 1u << (key[r] & 31u);
+                if ((*reinterpret_cast<volatile uint32_t*>(word) & bit) == 0u) atomicOr(word, bit);
+            }
         }
     }
+    for (int pass = 0; pass < passes; ++pass) {
+        const int shift = pass * 8;
+        uint32_t* out = buffers + (pass & 1) * 2 * chunk;
+        if (pass > 0) {
+            const uint32_t* in = buffers + ((pass - 1) & 1) * 2 * chunk;
+#pragma unroll
+            for (int r = 0; r < IT; ++r) {
+                const int i = mine + r * 32;
+                if (i < count) {
+                    key[r] = in[i];
+                    pos[r] = in[chunk + i];
+                }
+            }
+        }
+        for (int i = threadIdx.x; i < 32 * 256; i += 1024) counts[i] = 0u;
+        __syncthreads();
+        uint32_t at[IT];
+#pragma unroll
+        for (int r = 0; r < IT; ++r) {
+            const bool in = mine + r * 32 < count;
+            const uint32_t digit = in ? (key[r] >> shift) & 255u : 256u;
+            const uint32_t same = __match_any_sync(0xffffffffu, digit);
+            const uint32_t before = in ? counts[warp * 256 + digit] : 0u;
+            at[r] = before + __popc(same & ((1u << lane) - 1u));
+            __syncwarp();
+            if (in && (same >> lane) == 1u) counts[warp * 256 + digit] = before + __popc(same);
+            __syncwarp();
+        }
+        __syncthreads();
+        if (threadIdx.x < 256) {                           // over this CTA's warps
+            uint32_t sum = 0;
+#pragma unroll 8
+            for (int w = 0; w < 32; ++w) {
+                const uint32_t c = counts[w * 256 + threadIdx.x];
+                counts[w * 256 + threadIdx.x] = sum;
+                sum += c;
+            }
+            total[threadIdx.x] = sum;
+        }
+        __syncthreads();
+        cluster_sync();
+        if (threadIdx.x < 256) {                           // over the CTAs, then over the digits
+            uint32_t before = 0, all = 0;
+            for (int q = 0; q < ranks; ++q) {
+                const uint32_t c = ld_cluster_u32(mapa_shared(total + threadIdx.x, q));
+                before += q < rank ? c : 0u;
+                all += c;
+            }
+            uint32_t s = all;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t up = __shfl_up_sync(0xffffffffu, s, o);
+                if (lane >= o) s += up;
+            }
+            if (lane == 31) scan[warp] = s;
+            base[threadIdx.x] = s - all + before;
+        }
+        __syncthreads();
+        if (threadIdx.x < 256) {
+            uint32_t lower = 0;
+            for (int w = 0; w < warp; ++w) lower += scan[w];
+            base[threadIdx.x] += lower;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < IT; ++r) {
+            if (mine + r * 32 < count) {
+                const uint32_t digit = (key[r] >> shift) & 255u;
+                const uint32_t to = base[digit] + counts[warp * 256 + digit] + at[r];
+                if (pass + 1 == passes) {
+                    keys_out[to] = key[r];
+                    pos_out[to] = pos[r];
+                } else {
+                    const uint32_t q = to / static_cast<uint32_t>(chunk);
+                    const uint32_t local = mapa_shared(out + (to - q * chunk), q);
+                    st_cluster_u32(local, key[r]);
+                    st_cluster_u32(local + 4u * chunk, pos[r]);
+                }
+            }
+        }
+        cluster_sync();  // the list is complete, and nobody leaves or reuses what others read
+    }
 }
+
+// ---- the sums --------------------------------------------------------------------------------
 
 // A thread's four columns of a piece: neighbours where every row can be read 16 bytes at a time
 // (`vec`), else 256 apart, so that a warp still covers whole lines.
@@ -259,17 +386,37 @@ __device__ __forceinline__ void embed_store(float* p, int c0, int d, int vec, fl
 
 constexpr int kEmbedMaxWindow = 256;
 
-// One block per window of `window` sorted tokens and piece of 1024 columns. A run of one id that
-// lies inside the window is written out; the part of a run that came in from the window before
-// goes to part[2 w], the part of one that only goes on into the next to part[2 w + 1].
+// The first `sum_blocks` blocks: one per window of `window` sorted tokens and piece of 1024
+// columns. A run of one id that lies inside the window is written out; the part of a run that came
+// in from the window before goes to part[2 w], the part of one that only goes on into the next to
+// part[2 w + 1]. The blocks behind them write zeros into the rows that no token names, a warp per
+// row: they fill the memory system while the sums wait for their rows.
 __global__ void __launch_bounds__(256)
     embed_sum_kernel(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
                      long long n, int window, uint32_t rows, const float* __restrict__ grad,
                      long long ld_grad, int d, float scale, float* __restrict__ out, long long ld,
-                     float* __restrict__ part, int vec) {
+                     float* __restrict__ part, int vec, int pieces, int sum_blocks,
+                     const uint32_t* __restrict__ present) {
+    if (static_cast<int>(blockIdx.x) >= sum_blocks) {
+        const int lane = threadIdx.x & 31;
+        const int warps = (static_cast<int>(gridDim.x) - sum_blocks) * 8;
+        const int mine = (static_cast<int>(blockIdx.x) - sum_blocks) * 8 +
+                         static_cast<int>(threadIdx.x >> 5);
+        for (long long v = mine; v < rows; v += warps) {
+            if ((present[v >> 5] >> (v & 31)) & 1u) continue;
+            float* p = out + v * ld;
+            if (vec) {
+                for (int c = lane * 4; c < d; c += 128)
+                    *reinterpret_cast<float4*>(p + c) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            } else {
+                for (int c = lane; c < d; c += 32) p[c] = 0.0f;
+            }
+        }
+        return;
+    }
     __shared__ uint32_t s_key[kEmbedMaxWindow + 1], s_pos[kEmbedMaxWindow];
-    const long long w = blockIdx.x;
-    const int c0 = blockIdx.y * kEmbedPiece;
+    const long long w = static_cast<int>(blockIdx.x) / pieces;
+    const int c0 = (static_cast<int>(blockIdx.x) - static_cast<int>(w) * pieces) * kEmbedPiece;
     const long long first = w * window;
     const int count = static_cast<int>(min(static_cast<long long>(window), n - first));
     for (int i = threadIdx.x; i < count; i += 256) {

@@ -27,6 +27,52 @@ int launch_embedding(const float* table, int64_t rows, int64_t d, int64_t ld, co
     return MFK_OK;
 }
 
+template <typename ID, int IT>
+int launch_cluster_sort_it(const ID* ids, int64_t n, int ranks, int chunk, int64_t rows,
+                           int64_t padding, int passes, uint32_t* marks, uint32_t* keys,
+                           uint32_t* pos, int device, cudaStream_t stream) {
+    auto kernel = mfk::embed_sort_kernel<ID, IT>;
+    const int smem = (4 * chunk + 32 * 256 + 2 * 256 + 8) * 4;
+    static std::atomic<uint64_t> ready{0};  // a bit per device
+    if ((ready.load() >> device & 1u) == 0u) {
+        MFK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (4 * IT * 1024 + 32 * 256 + 2 * 256 + 8) * 4));
+        ready.fetch_or(uint64_t(1) << device);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3(static_cast<unsigned>(ranks), 1, 1);
+    cfg.blockDim = dim3(1024, 1, 1);
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cfg.stream = stream;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(ranks);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    MFK_CUDA(cudaLaunchKernelEx(&cfg, kernel, ids, static_cast<int>(n), chunk,
+                                static_cast<long long>(rows), static_cast<long long>(padding),
+                                passes, marks, keys, pos));
+    g_launches.fetch_add(1);
+    return MFK_OK;
+}
+
+// A cluster of CTAs with 2048 tokens each, or up to 8192 where eight CTAs need that.
+template <typename ID>
+int launch_cluster_sort(const ID* ids, int64_t n, int64_t rows, int64_t padding, int passes,
+                        uint32_t* marks, uint32_t* keys, uint32_t* pos, int device,
+                        cudaStream_t stream) {
+    const int ranks = static_cast<int>(
+        std::min<int64_t>(mfk::kClusterSortRanks, (n + 2047) / 2048));
+    const int chunk = static_cast<int>((n + ranks - 1) / ranks);
+    if (chunk <= 2048)
+        return launch_cluster_sort_it<ID, 2>(ids, n, ranks, chunk, rows, padding, passes, marks,
+                                             keys, pos, device, stream);
+    return launch_cluster_sort_it<ID, 8>(ids, n, ranks, chunk, rows, padding, passes, marks, keys,
+                                         pos, device, stream);
+}
+
 int run_embedding_grad(const float* grad, int64_t n, int64_t d, int64_t ld_grad, const void* ids,
                        int32_t id_bytes, int64_t rows, float scale, int64_t padding, float* out,
                        int64_t ld, cudaStream_t stream) {
@@ -45,13 +91,13 @@ int run_embedding_grad(const float* grad, int64_t n, int64_t d, int64_t ld_grad,
     const int vec = d % 4 == 0 && ld % 4 == 0 && ld_grad % 4 == 0 && aligned16(grad) &&
                     aligned16(out);
     const int pieces = static_cast<int>((d + mfk::kEmbedPiece - 1) / mfk::kEmbedPiece);
-    // windows: about eight blocks per SM, of 16 to 256 tokens
+    // windows of 16 to 256 tokens: three blocks per SM or more, and short joins of long runs
     int window = 16;
-    while (window < mfk::kEmbedMaxWindow && n * pieces / (window * 2) >= info->sm_count * 8)
+    while (window < mfk::kEmbedMaxWindow && n * pieces / (window * 2) >= info->sm_count * 3)
         window *= 2;
     const int64_t windows = (n + window - 1) / window;
     const int tiles = static_cast<int>((n + mfk::kSortTile - 1) / mfk::kSortTile);
-    if (windows > (int64_t(1) << 31) - 1 || pieces > 65535) return MFK_ERR_UNSUPPORTED;
+    if (windows * pieces > (int64_t(1) << 30) || pieces > 65535) return MFK_ERR_UNSUPPORTED;
 
     // one allocation: keys and positions twice, digit counts, the marks, the partial rows
     const size_t items = (static_cast<size_t>(n) + 63) / 64 * 64;
@@ -72,44 +118,55 @@ int run_embedding_grad(const float* grad, int64_t n, int64_t d, int64_t ld_grad,
     uint32_t* pos[2] = {words + 2 * items, words + 3 * items};
     uint32_t* d_counts = words + 4 * items;
     uint32_t* d_marks = d_counts + counts;
-    MFK_CUDA(cudaMemsetAsync(d_marks, 0, marks * 4, stream));
-
-    if (id_bytes == 8) {
-        mfk::embed_keys_kernel<int64_t><<<tiles, 256, 0, stream>>>(
-            static_cast<const int64_t*>(ids), n, rows, padding, keys[0], d_marks, d_counts, tiles);
-    } else {
-        mfk::embed_keys_kernel<int32_t><<<tiles, 256, 0, stream>>>(
-            static_cast<const int32_t*>(ids), n, rows, padding, keys[0], d_marks, d_counts, tiles);
-    }
-    g_launches.fetch_add(1);
-    const int64_t zero_blocks = std::min<int64_t>((rows + 7) / 8, int64_t(info->sm_count) * 64);
-    mfk::embed_zero_kernel<<<static_cast<unsigned>(zero_blocks), 256, 0, stream>>>(
-        d_marks, rows, static_cast<int>(d), out, ld, vec);
-    g_launches.fetch_add(1);
+    int passes = 0;
+    while (passes < 4 && (rows >> (passes * 8)) != 0) ++passes;
     int at = 0;
-    for (int shift = 0; shift < 32 && (rows >> shift) != 0; shift += 8) {
-        if (shift > 0) {
-            mfk::sort_count_kernel<<<tiles, 256, 0, stream>>>(keys[at], n, shift, d_counts, tiles);
-            g_launches.fetch_add(1);
+    if (n <= mfk::kClusterSortMax) {
+        rc = id_bytes == 8 ? launch_cluster_sort(static_cast<const int64_t*>(ids), n, rows, padding,
+                                                 passes, d_marks, keys[0], pos[0], dev, stream)
+                           : launch_cluster_sort(static_cast<const int32_t*>(ids), n, rows, padding,
+                                                 passes, d_marks, keys[0], pos[0], dev, stream);
+        if (rc != MFK_OK) return rc;
+    } else {
+        MFK_CUDA(cudaMemsetAsync(d_marks, 0, marks * 4, stream));
+        if (id_bytes == 8) {
+            mfk::embed_keys_kernel<int64_t><<<tiles, 256, 0, stream>>>(
+                static_cast<const int64_t*>(ids), n, rows, padding, keys[0], d_marks, d_counts,
+                tiles);
+        } else {
+            mfk::embed_keys_kernel<int32_t><<<tiles, 256, 0, stream>>>(
+                static_cast<const int32_t*>(ids), n, rows, padding, keys[0], d_marks, d_counts,
+                tiles);
         }
-        mfk::sort_scan_kernel<<<1, 1024, 0, stream>>>(d_counts, static_cast<int64_t>(counts));
-        mfk::sort_scatter_kernel<<<tiles, 256, 0, stream>>>(keys[at],
-                                                            shift > 0 ? pos[at] : nullptr, n, shift,
-                                                            d_counts, tiles, keys[at ^ 1],
-                                                            pos[at ^ 1]);
-        g_launches.fetch_add(2);
-        at ^= 1;
+        g_launches.fetch_add(1);
+        for (int pass = 0; pass < passes; ++pass) {
+            if (pass > 0) {
+                mfk::sort_count_kernel<<<tiles, 256, 0, stream>>>(keys[at], n, pass * 8, d_counts,
+                                                                  tiles);
+                g_launches.fetch_add(1);
+            }
+            mfk::sort_scan_kernel<<<1, 1024, 0, stream>>>(d_counts, static_cast<int64_t>(counts));
+            mfk::sort_scatter_kernel<<<tiles, 256, 0, stream>>>(
+                keys[at], pass > 0 ? pos[at] : nullptr, n, pass * 8, d_counts, tiles, keys[at ^ 1],
+                pos[at ^ 1]);
+            g_launches.fetch_add(2);
+            at ^= 1;
+        }
     }
-    const dim3 grid(static_cast<unsigned>(windows), static_cast<unsigned>(pieces), 1);
-    mfk::embed_sum_kernel<<<grid, 256, 0, stream>>>(keys[at], pos[at], n, window,
-                                                    static_cast<uint32_t>(rows), grad, ld_grad,
-                                                    static_cast<int>(d), scale, out, ld, d_part,
-                                                    vec);
-    mfk::embed_join_kernel<<<grid, 256, 0, stream>>>(keys[at], n, window,
-                                                     static_cast<uint32_t>(rows),
-                                                     static_cast<int>(d), scale, out, ld, d_part,
-                                                     vec);
-    g_launches.fetch_add(2);
+    const int sum_blocks = static_cast<int>(windows * pieces);
+    const int64_t zero_blocks = std::min<int64_t>((rows + 7) / 8, int64_t(info->sm_count) * 64);
+    mfk::embed_sum_kernel<<<static_cast<unsigned>(sum_blocks + zero_blocks), 256, 0, stream>>>(
+        keys[at], pos[at], n, window, static_cast<uint32_t>(rows), grad, ld_grad,
+        static_cast<int>(d), scale, out, ld, d_part, vec, pieces, sum_blocks, d_marks);
+    g_launches.fetch_add(1);
+    if (windows > 1) {
+        const dim3 grid(static_cast<unsigned>(windows), static_cast<unsigned>(pieces), 1);
+        mfk::embed_join_kernel<<<grid, 256, 0, stream>>>(keys[at], n, window,
+                                                         static_cast<uint32_t>(rows),
+                                                         static_cast<int>(d), scale, out, ld,
+                                                         d_part, vec);
+        g_launches.fetch_add(1);
+    }
     MFK_CUDA(cudaGetLastError());
     return MFK_OK;
 }

@@ -28,7 +28,8 @@ def close(got, grad, ids, rows, scale, padding=None):
 
 
 SIZES = [(1, 1, 1), (3, 5, 7), (64, 32, 129), (100, 1000, 64), (513, 300, 1003), (2049, 70000, 33),
-         (5000, 17, 260), (4096, 40, 1024), (9000, 1, 516), (20000, 257, 96)]
+         (5000, 17, 260), (4096, 40, 1024), (9000, 1, 516), (20000, 257, 96),
+         (16384, 300, 8), (30000, 70000, 36), (65536, 1000, 5), (65537, 1000, 5), (100000, 17000000, 1)]
 
 
 @pytest.mark.parametrize("n,rows,d", SIZES)
