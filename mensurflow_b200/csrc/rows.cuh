@@ -37,14 +37,6 @@ struct RowsArgs {
     int wait;                // x comes from the launch before
 };
 
-__device__ __forceinline__ void grid_dependents_go() {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-
-__device__ __forceinline__ void grid_wait() {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-
 __device__ __forceinline__ uint32_t cluster_nctarank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));

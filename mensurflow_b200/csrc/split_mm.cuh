@@ -154,6 +154,16 @@ __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool a_mn_major, 
            ((static_cast<uint32_t>(n) >> 3) << 17) | ((static_cast<uint32_t>(m) >> 4) << 24);
 }
 
+// Programmatic dependent launch: the launches of one call start while the one before still runs,
+// set themselves up, and wait for its results here.
+__device__ __forceinline__ void grid_dependents_go() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+__device__ __forceinline__ void grid_wait() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 __device__ __forceinline__ void prefetch_l2(const void* p) {
     asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
 }
@@ -240,6 +250,7 @@ struct XSources {
 // 128-byte row pieces and writes whole 128-byte core matrices. Bound by HBM: 4 bytes read, 4
 // written per entry.
 __global__ void __launch_bounds__(256) split_blocks_kernel(const __grid_constant__ XSources list) {
+    grid_dependents_go();
     int which = 0;
 #pragma unroll
     for (int i = 1; i < kXMaxSources; ++i)
@@ -333,6 +344,8 @@ __global__ void __launch_bounds__(256) split_blocks_kernel(const __grid_constant
 __global__ void __launch_bounds__(256) split_normalize_kernel(const double* sumsq, float* inv,
                                                               int blocks, float eps) {
     __shared__ double part[256];
+    grid_dependents_go();
+    grid_wait();
     const double* p = sumsq + static_cast<long long>(blockIdx.x) * blocks;
     double sum = 0.0;
     for (int i = threadIdx.x; i < blocks; i += 256) sum += p[i];
@@ -994,6 +1007,7 @@ __global__ void __launch_bounds__(kXThreads, 1)
     const uint32_t rank = CG == 1 ? 0u : cluster_ctarank();
     const int first = static_cast<int>(blockIdx.x) / CG, step = static_cast<int>(gridDim.x) / CG;
 
+    grid_dependents_go();
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::kStages; ++s) {
             mbar_init(&full[s], 1);
@@ -1023,6 +1037,7 @@ __global__ void __launch_bounds__(kXThreads, 1)
     if constexpr (CG == 2) cluster_sync();
     tc_fence_after();
     const uint32_t tmem = *tmem_holder;
+    grid_wait();  // before anything of the launch before is read or overwritten
 
     if (warp == 0) {
         if (lane == 0)
