@@ -23,6 +23,7 @@
 #include "embed.cuh"
 #include "gemm_tc.cuh"
 #include "movement.cuh"
+#include "orth_small.cuh"
 #include "prep.cuh"
 #include "rows.cuh"
 #include "simt.cuh"

@@ -34,6 +34,7 @@ def close(got, ref, steps=5):
 
 
 SIZES = [(1, 1), (1, 7), (9, 1), (2, 3), (64, 64), (64, 128), (127, 129), (128, 128), (130, 64),
+         (128, 1024), (1024, 100), (1000, 128), (65, 640), (128, 1025), (1030, 90),
          (256, 200), (257, 513), (700, 300), (384, 1500), (1003, 771)]
 
 
@@ -44,4 +45,18 @@ def test_sizes(cuda, shape):
     got = mf.orthogonalize(u)
     assert got.shape == u.shape
     close(got, want(u))
+    assert mf.device_status() == 0
+
+
+@pytest.mark.parametrize("shape", [(3, 64, 128), (300, 16, 40), (2, 3, 128, 257), (5, 200, 130),
+                                   (40, 600, 100)])
+def test_batches(cuda, shape):
+    g = torch.Generator(device="cuda").manual_seed(sum(shape))
+    u = torch.randn(*shape, generator=g, device=cuda)
+    u = u * torch.logspace(-6, 6, shape[0], device=cuda).reshape(-1, *[1] * (len(shape) - 1))
+    got = mf.orthogonalize(u)
+    assert got.shape == u.shape
+    close(got, want(u))
+    alone = torch.stack([mf.orthogonalize(m) for m in u])     # a batch is its matrices
+    close(alone, want(u))
     assert mf.device_status() == 0
