@@ -11,7 +11,7 @@
 // once, the table written once.
 #pragma once
 
-#include "mfk_ptx.cuh"
+#include "split_mm.cuh"
 
 namespace mfk {
 
@@ -214,12 +214,6 @@ constexpr int kClusterSortMax = kClusterSortRanks * 8192;   // tokens
 
 __device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-}
-
-__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
-    uint32_t v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-    return v;
 }
 
 // Up to 65536 tokens in one cluster of up to 8 CTAs: each holds `chunk` of the list in shared

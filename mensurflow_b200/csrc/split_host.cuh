@@ -5,7 +5,7 @@
 
 namespace {
 
-constexpr int kXKinds = 12;  // kernel instantiations with per-device set-up
+constexpr int kXKinds = 48;  // kernel instantiations (and cluster sizes) with per-device set-up
 
 struct XDevice {
     bool ready[kXKinds] = {};
@@ -23,16 +23,14 @@ struct XMat {
     int64_t blocks() const { return static_cast<int64_t>(rb) * cb; }
 };
 
-// One stream-ordered allocation: all split blocks, their 1/s, sums of squares, partial sums and
-// counters of split contractions.
+// One stream-ordered allocation: all split blocks, their 1/s, sums of squares, and what else a call
+// asks for.
 struct XWorkspace {
     cudaStream_t stream;
     uint8_t* base = nullptr;
     uint8_t* blocks = nullptr;
     float* inv = nullptr;
     double* sumsq = nullptr;
-    float* part = nullptr;
-    int* count = nullptr;
     float* extra = nullptr;
     int64_t total_blocks = 0;
     CUtensorMap mk, mm;
@@ -46,10 +44,6 @@ struct XWorkspace {
         if (base != nullptr) cudaFreeAsync(base, stream);
     }
 };
-
-// Partial sums of split contractions: at most kXMaxParts CTA accumulators of 128 x 256.
-constexpr int kXMaxParts = 320;
-constexpr int kXMaxCounters = 1024;
 
 XMat x_mat(XWorkspace& ws, int64_t rows, int64_t cols, int64_t batch = 1) {
     XMat m;
@@ -79,10 +73,7 @@ int x_allocate(XWorkspace& ws, size_t extra_floats) {
     const size_t block_bytes = static_cast<size_t>(ws.total_blocks) * mfk::kXBlockBytes;
     const size_t inv_bytes = (static_cast<size_t>(ws.total_blocks) * 4 + 255) / 256 * 256;
     const size_t sum_bytes = (static_cast<size_t>(ws.total_blocks) * 8 + 255) / 256 * 256;
-    const size_t part_bytes = static_cast<size_t>(kXMaxParts) * 128 * 256 * 4;
-    const size_t count_bytes = kXMaxCounters * sizeof(int);
-    const size_t total = block_bytes + inv_bytes + sum_bytes + part_bytes + count_bytes +
-                         extra_floats * 4 + 1024;
+    const size_t total = block_bytes + inv_bytes + sum_bytes + extra_floats * 4 + 1024;
     MFK_CUDA(cudaMallocAsync(reinterpret_cast<void**>(&ws.base), total, ws.stream));
     uint8_t* p = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ws.base) + 1023) &
                                             ~static_cast<uintptr_t>(1023));
@@ -92,12 +83,7 @@ int x_allocate(XWorkspace& ws, size_t extra_floats) {
     p += inv_bytes;
     ws.sumsq = reinterpret_cast<double*>(p);
     p += sum_bytes;
-    ws.part = reinterpret_cast<float*>(p);
-    p += part_bytes;
-    ws.count = reinterpret_cast<int*>(p);
-    p += count_bytes;
     ws.extra = reinterpret_cast<float*>(p);
-    MFK_CUDA(cudaMemsetAsync(ws.count, 0, count_bytes, ws.stream));
     // The blocks as 2 KB lines of 256 eight-byte units. K-major stages take 8 whole lines,
     // MN-major ones the same 1 KB of 16 lines.
     auto fn = encode_fn();
@@ -175,24 +161,25 @@ mfk::XOut x_out(const XWorkspace& ws, const XMat& m) {
     return o;
 }
 
-template <int CG, int NB, int EPI>
-int x_slots(XWorkspace& ws, int kind, int* slots) {
+// CTAs, pairs or clusters of `cluster` CTAs of a kernel that the device holds at once.
+template <int CG, int NB, int EPI, bool SPL>
+int x_slots(XWorkspace& ws, int kind, int cluster, int* slots) {
     using C = mfk::XConfig<CG, NB>;
-    auto kernel = mfk::split_mm_kernel<CG, NB, EPI>;
+    auto kernel = mfk::split_mm_kernel<CG, NB, EPI, SPL>;
     std::lock_guard<std::mutex> lock(g_mutex);
     XDevice& d = g_xdevices[ws.dev];
     if (!d.ready[kind]) {
         MFK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       C::kSmemBytes));
-        int n = ws.info->sm_count / CG;
-        if (CG > 1) {
+        int n = ws.info->sm_count / cluster;
+        if (cluster > 1) {
             cudaLaunchConfig_t cfg = {};
             cudaLaunchAttribute attr[1];
             cfg.blockDim = dim3(mfk::kXThreads, 1, 1);
-            cfg.gridDim = dim3(static_cast<unsigned>(n * CG), 1, 1);
+            cfg.gridDim = dim3(static_cast<unsigned>(n * cluster), 1, 1);
             cfg.dynamicSmemBytes = C::kSmemBytes;
             attr[0].id = cudaLaunchAttributeClusterDimension;
-            attr[0].val.clusterDim.x = CG;
+            attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
             attr[0].val.clusterDim.y = 1;
             attr[0].val.clusterDim.z = 1;
             cfg.attrs = attr;
@@ -210,34 +197,29 @@ int x_slots(XWorkspace& ws, int kind, int* slots) {
     return MFK_OK;
 }
 
-// Time of one launch in SM cycles, and the contraction split that gives the least of it. A chunk
-// of 128 takes 24 MMAs: 3072 cycles for a pair's 256 x 256 (or one CTA's 128 x 256), 1536 for
-// 128 x 128. A split adds the exchange of partial sums through L2.
-double x_cost(int64_t tiles, int slots, double chunk, int kc, int nb, int64_t max_parts,
-              int cta_group, int* splits) {
-    double best = 0.0;
-    *splits = 0;
-    for (int s = 1; s <= kc && s <= 32; ++s) {
-        if (s > 1 && (tiles * s * cta_group > max_parts || tiles * cta_group > kXMaxCounters))
-            break;
-        const int64_t waves = (tiles * s + slots - 1) / slots;
-        double t = static_cast<double>(waves) * ((kc + s - 1) / s * chunk + 1500.0 * nb);
-        if (s > 1) t += 4000.0 + 1100.0 * nb * s;
-        if (*splits == 0 || t < best) {
-            best = t;
-            *splits = s;
-        }
-    }
-    return best;
+// Time of a launch in SM cycles: whole waves of tiles, and the part of the epilogue that no product
+// hides. A chunk of 128 takes 24 MMAs: 3072 cycles for a pair's 256 x 256, which it reaches (its
+// 128 KB per CTA come at 42 bytes a cycle). One CTA's 128 x 128 would take 1536, but 128 KB in that
+// time is more than an SM gets from L2: 2500 measured (4 to 50 chunks), and 4200 for 128 x 256.
+// Sharing a contraction costs 9000 cycles (128 x 128) or 17000 per wave (1024 x 1024 over a depth
+// of 1024: 15.6 us by clusters of 3 single CTAs, 24.5 us by clusters of 4 pairs).
+double x_cost(int64_t tiles, int slots, double chunk, int kc, double epilogue) {
+    const int64_t waves = (tiles + slots - 1) / slots;
+    return static_cast<double>(waves) * (kc * chunk + epilogue);
 }
 
-template <int CG, int NB, int EPI>
-int x_launch_kind(XWorkspace& ws, mfk::XArgs& g, int slots, int batch) {
+template <int CG, int NB, int EPI, bool SPL>
+int x_launch(XWorkspace& ws, mfk::XArgs& g, int slots, int64_t batch, int64_t tm, int64_t tn,
+             int64_t tiles, int splits) {
     using C = mfk::XConfig<CG, NB>;
-    auto kernel = mfk::split_mm_kernel<CG, NB, EPI>;
-    g.units = g.tiles * batch * g.splits;
-    const int units = std::min(g.units, slots);
-    // (4096 x 1024 x 4096: 15 products of the update in a row, 396 us without the overlap)
+    auto kernel = mfk::split_mm_kernel<CG, NB, EPI, SPL>;
+    g.tiles_m = static_cast<int>(tm);
+    g.tiles_n = static_cast<int>(tn);
+    g.tiles = static_cast<int>(tiles);
+    g.splits = splits;
+    g.units = static_cast<int>(tiles * batch) * splits;
+    const int cluster = CG * splits;
+    const int units = SPL ? g.units : std::min(g.units, slots);
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     cfg.blockDim = dim3(mfk::kXThreads, 1, 1);
@@ -247,11 +229,11 @@ int x_launch_kind(XWorkspace& ws, mfk::XArgs& g, int slots, int batch) {
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = CG;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = CG > 1 ? 2 : 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     {
         TimedLaunch timed(ws.stream);
         MFK_CUDA(cudaLaunchKernelEx(&cfg, kernel, ws.mk, ws.mm, g));
@@ -268,37 +250,49 @@ int x_product(XWorkspace& ws, mfk::XArgs& g, int64_t k0, int64_t k1, int64_t bat
     g.kc = g.kc0 + static_cast<int>((k1 + mfk::kXBlk - 1) / mfk::kXBlk);
     g.last0 = (k0 - 1) % mfk::kXBlk < 64 ? 1 : 2;
     g.last1 = k1 > 0 ? ((k1 - 1) % mfk::kXBlk < 64 ? 1 : 2) : g.last0;
-    g.part = ws.part;
-    g.count = ws.count;
-    int slots2 = 0, slots1 = 0;
-    int rc = x_slots<2, 2, EPI>(ws, EPI * 2, &slots2);
-    if (rc != MFK_OK) return rc;
-    rc = x_slots<1, kNb1, EPI>(ws, EPI * 2 + 1, &slots1);
-    if (rc != MFK_OK) return rc;
-    // 256 x 256 by pairs of CTAs where there are tiles enough, 128-row tiles of one CTA where
-    // there are not.
     const int per_tile_n = EPI == mfk::kXGated ? 1 : 2;
     const int64_t tm2 = (g.mb + 1) / 2, tn2 = (g.nb + per_tile_n - 1) / per_tile_n;
     const int64_t tm1 = g.mb, tn1 = g.nb;
     const int64_t tiles2 = g.sym ? tm2 * (tm2 + 1) / 2 : tm2 * tn2;
     const int64_t tiles1 = g.sym ? tm1 * (tm1 + 1) / 2 : tm1 * tn1;
-    if (tiles1 * batch > (int64_t(1) << 30)) return MFK_ERR_UNSUPPORTED;
-    int s2 = 1, s1 = 1;
-    const double c2 = x_cost(tiles2 * batch, slots2, 3072.0, g.kc, 2, kXMaxParts, 2, &s2);
-    const double c1 = x_cost(tiles1 * batch, slots1, 1700.0 * kNb1, g.kc, kNb1,
-                             kXMaxParts * 2 / kNb1, 1, &s1);
-    if (c2 <= c1) {
-        g.tiles_m = static_cast<int>(tm2);
-        g.tiles_n = static_cast<int>(tn2);
-        g.tiles = static_cast<int>(tiles2);
-        g.splits = s2;
-        return x_launch_kind<2, 2, EPI>(ws, g, slots2, static_cast<int>(batch));
+    if (tiles1 * batch > (int64_t(1) << 26)) return MFK_ERR_UNSUPPORTED;
+    // The backward epilogue has three outputs and two inputs, the gated one an activation.
+    constexpr double kEpi = EPI == mfk::kXGatedBwd ? 12000.0 : EPI == mfk::kXGated ? 6000.0
+                                                                                   : 3000.0;
+    // 256 x 256 by pairs of CTAs where there are tiles enough, 128-row tiles of one CTA where there
+    // are not, and either with the contraction shared by a cluster where that leaves SMs idle.
+    int slots = 0, best_slots = 0, pairs = 0, splits = 0, rc = MFK_OK;
+    double least = 0.0;
+    auto consider = [&](int cta_group, int s, int64_t tiles, double chunk, double epilogue,
+                        double exchange) {
+        double t = x_cost(tiles * batch, slots, chunk, (g.kc + s - 1) / s, epilogue / s);
+        if (s > 1) t += exchange * static_cast<double>((tiles * batch + slots - 1) / slots);
+        if (splits == 0 || t < least) {
+            least = t;
+            pairs = cta_group - 1;
+            splits = s;
+            best_slots = slots;
+        }
+    };
+    for (int s = 1; s <= 4 && s <= g.kc; ++s) {
+        rc = s == 1 ? x_slots<2, 2, EPI, false>(ws, EPI * 12 + s - 1, 2, &slots)
+                    : x_slots<2, 2, EPI, true>(ws, EPI * 12 + s - 1, 2 * s, &slots);
+        if (rc != MFK_OK) return rc;
+        consider(2, s, tiles2, 3072.0, kEpi * 2, 17000.0);
     }
-    g.tiles_m = static_cast<int>(tm1);
-    g.tiles_n = static_cast<int>(tn1);
-    g.tiles = static_cast<int>(tiles1);
-    g.splits = s1;
-    return x_launch_kind<1, kNb1, EPI>(ws, g, slots1, static_cast<int>(batch));
+    for (int s = 1; s <= 8 && s <= g.kc; ++s) {
+        rc = s == 1 ? x_slots<1, kNb1, EPI, false>(ws, EPI * 12 + 3 + s, 1, &slots)
+                    : x_slots<1, kNb1, EPI, true>(ws, EPI * 12 + 3 + s, s, &slots);
+        if (rc != MFK_OK) return rc;
+        consider(1, s, tiles1, kNb1 == 2 ? 4200.0 : 2500.0, kEpi, kNb1 == 2 ? 17000.0 : 9000.0);
+    }
+    if (pairs)
+        return splits == 1
+                   ? x_launch<2, 2, EPI, false>(ws, g, best_slots, batch, tm2, tn2, tiles2, 1)
+                   : x_launch<2, 2, EPI, true>(ws, g, best_slots, batch, tm2, tn2, tiles2, splits);
+    return splits == 1
+               ? x_launch<1, kNb1, EPI, false>(ws, g, best_slots, batch, tm1, tn1, tiles1, 1)
+               : x_launch<1, kNb1, EPI, true>(ws, g, best_slots, batch, tm1, tn1, tiles1, splits);
 }
 
 int x_zero(float* out, int64_t rows, int64_t cols, int64_t ld, cudaStream_t stream) {

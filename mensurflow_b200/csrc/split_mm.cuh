@@ -79,8 +79,6 @@ struct XArgs {
     float* gmax;           // largest |gate|, |up| per block
     int act;
     int store_h;
-    float* part;           // partial accumulators of split contractions
-    int* count;
 };
 
 // ---- PTX forms this kernel adds --------------------------------------------------------------
@@ -158,6 +156,21 @@ __device__ __forceinline__ uint32_t cluster_nctarank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
     return r;
+}
+
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
 }
 
 // Programmatic dependent launch: the launches of one call start while the one before still runs,
@@ -524,7 +537,8 @@ __device__ __forceinline__ void x_load(uint8_t* dst, const CUtensorMap* mk, cons
 template <int CG, int NB, int EPI>
 __device__ __forceinline__ void x_producer(const XArgs& g, const CUtensorMap* mk,
                                            const CUtensorMap* mm, uint8_t* stages, uint64_t* full,
-                                           uint64_t* empty, uint32_t rank, int first, int step) {
+                                           uint64_t* empty, uint32_t rank, uint32_t leader,
+                                           int first, int step) {
     using C = XConfig<CG, NB>;
     int stage = 0;
     uint32_t phase = 0;
@@ -549,7 +563,7 @@ __device__ __forceinline__ void x_producer(const XArgs& g, const CUtensorMap* mk
                     mbar_arrive_expect_tx(&full[stage], C::kStageBytes);
                 } else {
                     if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * C::kStageBytes);
-                    bar0 = mapa_shared(&full[stage], 0);
+                    bar0 = mapa_shared(&full[stage], leader);
                 }
                 x_load<CG>(s, mk, mm, &full[stage], bar0, g.a[seg], w.z, w.tm * CG, i,
                            k, h);
@@ -577,7 +591,7 @@ __device__ __forceinline__ void x_producer(const XArgs& g, const CUtensorMap* mk
 template <int CG, int NB, int EPI>
 __device__ __forceinline__ void x_mma(const XArgs& g, uint32_t tmem, uint8_t* stages,
                                       uint64_t* full, uint64_t* empty, uint64_t* tfull,
-                                      uint64_t* tempty, int first, int step) {
+                                      uint64_t* tempty, uint32_t leader, int first, int step) {
     using C = XConfig<CG, NB>;
     constexpr int kM = 128 * CG;
     constexpr int kN = CG == 2 ? 128 * NB : 128;
@@ -632,7 +646,7 @@ __device__ __forceinline__ void x_mma(const XArgs& g, uint32_t tmem, uint8_t* st
                 if constexpr (CG == 1) {
                     mma_commit(&empty[stage]);
                 } else {
-                    mma_commit_cg2_mc(&empty[stage], 3);
+                    mma_commit_cg2_mc(&empty[stage], static_cast<uint16_t>(3u << leader));
                 }
                 if (++stage == C::kStages) {
                     stage = 0;
@@ -642,7 +656,7 @@ __device__ __forceinline__ void x_mma(const XArgs& g, uint32_t tmem, uint8_t* st
             if constexpr (CG == 1) {
                 mma_commit(&tfull[buf]);
             } else {
-                mma_commit_cg2_mc(&tfull[buf], 3);
+                mma_commit_cg2_mc(&tfull[buf], static_cast<uint16_t>(3u << leader));
             }
             if (++buf == 2) {
                 buf = 0;
@@ -662,10 +676,17 @@ __device__ __forceinline__ void x_max_into(uint32_t* red, float amax) {
 
 // Thread (quarter q, half h, lane) owns row 32 q + lane of the CTA's 128 and, of every 128-column
 // block of the tile, columns 64 h .. 64 h + 63: acc[64 b + j] is column 64 h + j of block b.
-template <int CG, int NB, int EPI>
-__device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* epi_smem, uint32_t* red,
-                                           int* last_flag, uint32_t tmem, uint64_t* tfull,
-                                           uint64_t* tempty, uint32_t rank, int first, int step) {
+//
+// SPL: the contraction is shared by g.splits CTAs (or pairs) of one cluster, one tile each. A CTA
+// leaves its sums in its own shared memory (the stages are read by then) and takes over its share
+// of each thread's eight groups of eight columns (at most four): it adds the cluster's sums of those, in rank order,
+// through distributed shared memory, and finishes them. (Through L2, with one CTA adding and
+// finishing everything, the exchange took 8 us of a 17 us product.)
+template <int CG, int NB, int EPI, bool SPL>
+__device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint8_t* epi_smem,
+                                           uint32_t* red, uint32_t tmem, uint64_t* tfull,
+                                           uint64_t* tempty, uint32_t rank, uint32_t leader,
+                                           int first, int step) {
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int q = warp % 4, half = (warp - kXEpiWarp0) / 4;
     const int row = q * 32 + lane;
@@ -683,7 +704,7 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* epi_smem, ui
             // the tile's gate and up into L2 while its product is computed
             for (int b = 0; b < NB; ++b) {
                 const int jb = w.tn * NB + b;
-                if (i < g.mb && jb < g.nb && w.s == g.splits - 1) {
+                if (i < g.mb && jb < g.nb && w.s == 0) {
                     const long long at = (static_cast<long long>(i) * g.o[0].ldb + jb) * 16384;
                     for (int x = et * 32; x < 16384; x += kXEpiThreads * 32) {
                         prefetch_l2(g.gate + at + x);
@@ -740,7 +761,7 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* epi_smem, ui
                 if constexpr (CG == 1) {
                     mbar_arrive(&tempty[buf]);
                 } else {
-                    mbar_arrive_cluster(mapa_shared(&tempty[buf], 0));
+                    mbar_arrive_cluster(mapa_shared(&tempty[buf], leader));
                 }
             }
             if (++buf == 2) {
@@ -748,35 +769,35 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* epi_smem, ui
                 tphase ^= 1u;
             }
         }
-        if (g.splits > 1) {
-            // A split contraction: every part leaves its sums, and the part that finds itself
-            // counted last adds them in the parts' order (the same sum whichever that is).
-            constexpr int kPart = NB * 64 * kXEpiThreads;
-            float* mine = g.part + (static_cast<long long>(u) * CG + rank) * kPart;
+        // this CTA's groups of eight columns: ng of them from ch0, at the front of acc
+        const int ch0 = SPL ? 8 * w.s / g.splits : 0;
+        const int ng = SPL ? 8 * (w.s + 1) / g.splits - ch0 : 8;
+        if constexpr (SPL) {
+            float4* mine = reinterpret_cast<float4*>(stages) + et;
 #pragma unroll
-            for (int j = 0; j < NB * 64; ++j) __stcg(mine + j * kXEpiThreads + et, acc[j]);
-            __threadfence();
-            epi_bar();
-            if (et == 0) {
-                int* n = g.count + w.tile * CG + rank;
-                const int before = atomicAdd(n, 1);
-                const int is_last = before == g.splits - 1 ? 1 : 0;
-                if (is_last) *n = 0;  // ready for the next launch
-                *last_flag = is_last;
-                __threadfence();
-            }
-            epi_bar();
-            const int is_last = *last_flag;
-            epi_bar();
-            if (!is_last) continue;
+            for (int j = 0; j < NB * 16; ++j)
+                mine[j * kXEpiThreads] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2],
+                                                     acc[4 * j + 3]);
+            cluster_sync();
 #pragma unroll
-            for (int j = 0; j < NB * 64; ++j) acc[j] = 0.0f;
-            for (int s = 0; s < g.splits; ++s) {
-                const float* p =
-                    g.part +
-                    ((static_cast<long long>(w.tile) * g.splits + s) * CG + rank) * kPart;
+            for (int b = 0; b < NB; ++b) {
 #pragma unroll
-                for (int j = 0; j < NB * 64; ++j) acc[j] += __ldcg(p + j * kXEpiThreads + et);
+                for (int ch = 0; ch < 8; ++ch) {
+                    float* v = acc + b * 64 + ch * 8;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+                    if (ch < 4 && ch < ng) {
+                        for (int r = 0; r < g.splits; ++r) {
+                            const uint32_t at = mapa_shared(
+                                mine + (b * 16 + (ch0 + ch) * 2) * kXEpiThreads,
+                                r * CG + rank);
+                            const float4 x = ld_cluster_v4(at);
+                            const float4 y = ld_cluster_v4(at + kXEpiThreads * 16);
+                            v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+                            v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
+                        }
+                    }
+                }
             }
         }
         const bool row_block = i < g.mb;
@@ -790,9 +811,10 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* epi_smem, ui
                     const int blk = w.z * g.c.bstride + i * g.c.ldb + jb;
                     const float f = g.c.inv[blk] * g.beta;
                     const uint8_t* p = g.c.data + static_cast<long long>(blk) * kXBlockBytes +
-                                       half * 8 * kXLineBytes + row * 16;
+                                       (half * 8 + ch0) * kXLineBytes + row * 16;
 #pragma unroll
                     for (int ch = 0; ch < 8; ++ch) {
+                        if (SPL && ch >= ng) break;
                         const uint4 hq = *reinterpret_cast<const uint4*>(p + ch * kXLineBytes);
                         const uint4 lq = *reinterpret_cast<const uint4*>(p + ch * kXLineBytes +
                                                                          kXBlockBytes / 2);
@@ -817,7 +839,30 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* epi_smem, ui
             }
         }
 
-        if constexpr (EPI == kXF32) {
+        if constexpr (EPI == kXF32 && SPL) {
+            const int grow = i * kXBlk + row;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+#pragma unroll
+                for (int ch = 0; ch < 4; ++ch) {
+                    const int col = (w.tn * NB + b) * kXBlk + half * 64 + (ch0 + ch) * 8;
+                    if (ch < ng && grow < g.m) {
+                        float* dst = g.out + w.z * g.out_bs +
+                                     static_cast<long long>(grow) * g.ld + col;
+                        const float* v = acc + b * 64 + ch * 8;
+                        if (col + 8 <= g.n && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
+                            *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+                            *reinterpret_cast<float4*>(dst + 4) =
+                                make_float4(v[4], v[5], v[6], v[7]);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                if (col + e < g.n) dst[e] = v[e];
+                        }
+                    }
+                }
+            }
+        } else if constexpr (EPI == kXF32) {
             // through a 32 x 32 box, so that a warp writes 32 consecutive columns of one row at a
             // time, whatever the row stride
 #pragma unroll
@@ -854,18 +899,29 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* epi_smem, ui
             parity = parity == 2 ? 0 : parity + 1;
             if (et < 4) red[parity * 4 + et] = 0u;
             epi_bar();
+            uint32_t top_of[3] = {slot[0], slot[1], slot[2]};
+            if constexpr (SPL) {
+                cluster_sync();
+                for (int r = 0; r < g.splits; ++r) {
+                    const uint32_t at = mapa_shared(slot, r * CG + rank);
+#pragma unroll
+                    for (int e = 0; e < 3; ++e)
+                        top_of[e] = max(top_of[e], ld_cluster_u32(at + e * 4));
+                }
+            }
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 const int jb = w.tn * NB + b;
                 if (row_block && jb < g.nb) {
                     const int blk = w.z * g.o[0].bstride + i * g.o[0].ldb + jb;
                     float s, inv;
-                    split_scale(__uint_as_float(slot[b]), s, inv);
-                    if (et == 0) g.o[0].inv[blk] = inv;
+                    split_scale(__uint_as_float(top_of[b]), s, inv);
+                    if (et == 0 && w.s == 0) g.o[0].inv[blk] = inv;
                     uint8_t* dst = g.o[0].data + static_cast<long long>(blk) * kXBlockBytes;
 #pragma unroll
                     for (int ch = 0; ch < 8; ++ch)
-                        store_split8(dst, half * 8 + ch, row, acc + b * 64 + ch * 8, s);
+                        if (ch < ng)
+                            store_split8(dst, half * 8 + ch0 + ch, row, acc + b * 64 + ch * 8, s);
                 }
             }
         }
@@ -878,12 +934,14 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* epi_smem, ui
                 x_max_into(slot + 1, largest<64>(acc));
                 x_max_into(slot + 2, largest<64>(acc + 64));
             }
-            const long long at = (static_cast<long long>(blk) * 2 + half) * 64 * kXBlk + row * 4;
+            const long long at =
+                ((static_cast<long long>(blk) * 2 + half) * 64 + ch0 * 8) * kXBlk + row * 4;
             const bool save = g.gate != nullptr && row_block;
             // the stores of the pre-activations go out between the activations' arithmetic
             with_act(g.store_h ? g.act : kXActNone, [&](auto kind) {
 #pragma unroll
                 for (int j = 0; j < 64; j += 4) {
+                    if (SPL && j >= ng * 8) break;
                     if (save) {
                         *reinterpret_cast<float4*>(g.gate + at + j * kXBlk) =
                             make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
@@ -899,19 +957,29 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* epi_smem, ui
             parity = parity == 2 ? 0 : parity + 1;
             if (et < 4) red[parity * 4 + et] = 0u;
             epi_bar();
+            uint32_t top_of[3] = {slot[0], slot[1], slot[2]};
+            if constexpr (SPL) {
+                cluster_sync();
+                for (int r = 0; r < g.splits; ++r) {
+                    const uint32_t at = mapa_shared(slot, r * CG + rank);
+#pragma unroll
+                    for (int e = 0; e < 3; ++e)
+                        top_of[e] = max(top_of[e], ld_cluster_u32(at + e * 4));
+                }
+            }
             if (row_block) {
-                if (g.gate != nullptr && et == 0) {
-                    g.gmax[blk * 2] = __uint_as_float(slot[1]);
-                    g.gmax[blk * 2 + 1] = __uint_as_float(slot[2]);
+                if (g.gate != nullptr && et == 0 && w.s == 0) {
+                    g.gmax[blk * 2] = __uint_as_float(top_of[1]);
+                    g.gmax[blk * 2 + 1] = __uint_as_float(top_of[2]);
                 }
                 if (g.store_h) {
                     float s, inv;
-                    split_scale(__uint_as_float(slot[0]), s, inv);
-                    if (et == 0) g.o[0].inv[blk] = inv;
+                    split_scale(__uint_as_float(top_of[0]), s, inv);
+                    if (et == 0 && w.s == 0) g.o[0].inv[blk] = inv;
                     uint8_t* dst = g.o[0].data + static_cast<long long>(blk) * kXBlockBytes;
 #pragma unroll
                     for (int ch = 0; ch < 8; ++ch)
-                        store_split8(dst, half * 8 + ch, row, acc + ch * 8, s);
+                        if (ch < ng) store_split8(dst, half * 8 + ch0 + ch, row, acc + ch * 8, s);
                 }
             }
         }
@@ -929,25 +997,36 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* epi_smem, ui
             parity = parity == 2 ? 0 : parity + 1;
             if (et < 4) red[parity * 4 + et] = 0u;
             epi_bar();
+            uint32_t top_of[3] = {slot[0], slot[1], slot[2]};
+            if constexpr (SPL) {
+                cluster_sync();
+                for (int r = 0; r < g.splits; ++r) {
+                    const uint32_t at = mapa_shared(slot, r * CG + rank);
+#pragma unroll
+                    for (int e = 0; e < 3; ++e)
+                        top_of[e] = max(top_of[e], ld_cluster_u32(at + e * 4));
+                }
+            }
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 const int jb = w.tn * NB + b;
                 if (row_block && jb < g.nb) {
                     const int blk = i * g.o[0].ldb + jb;
-                    const float dm = __uint_as_float(slot[b]);
+                    const float dm = __uint_as_float(top_of[b]);
                     const float gm = g.gmax[blk * 2], um = g.gmax[blk * 2 + 1];
                     float s0, s1, s2, i0, i1, i2;
                     const float top = 3.402823466e38f;
                     split_scale(fminf(dm * um * kXMaxSlope, top), s0, i0);
                     split_scale(fminf(dm * gm, top), s1, i1);
                     split_scale(fminf(gm * um, top), s2, i2);
-                    if (et == 0) {
+                    if (et == 0 && w.s == 0) {
                         g.o[0].inv[blk] = i0;
                         g.o[1].inv[blk] = i1;
                         g.o[2].inv[blk] = i2;
                     }
                     const long long at =
-                        (static_cast<long long>(blk) * 2 + half) * 64 * kXBlk + row * 4;
+                        ((static_cast<long long>(blk) * 2 + half) * 64 + ch0 * 8) * kXBlk +
+                        row * 4;
                     const long long off = static_cast<long long>(blk) * kXBlockBytes;
 with_act(g.act, [&](auto kind) {
                     float4 gv[2], uv[2];  // eight columns, loaded one turn ahead
@@ -958,12 +1037,13 @@ with_act(g.act, [&](auto kind) {
                     }
 #pragma unroll
                     for (int ch = 0; ch < 8; ++ch) {
+                        if (SPL && ch >= ng) break;
                         float dg[8], du[8], hh[8];
                         const float gs[8] = {gv[0].x, gv[0].y, gv[0].z, gv[0].w,
                                              gv[1].x, gv[1].y, gv[1].z, gv[1].w};
                         const float us[8] = {uv[0].x, uv[0].y, uv[0].z, uv[0].w,
                                              uv[1].x, uv[1].y, uv[1].z, uv[1].w};
-                        if (ch < 7) {
+                        if (ch + 1 < ng) {
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
                                 const long long x = at + (ch * 8 + 8 + e * 4) * kXBlk;
@@ -979,18 +1059,19 @@ with_act(g.act, [&](auto kind) {
                             du[x] = dh * as.x;
                             hh[x] = as.x * us[x];
                         }
-                        store_split8(g.o[0].data + off, half * 8 + ch, row, dg, s0);
-                        store_split8(g.o[1].data + off, half * 8 + ch, row, du, s1);
-                        store_split8(g.o[2].data + off, half * 8 + ch, row, hh, s2);
+                        store_split8(g.o[0].data + off, half * 8 + ch0 + ch, row, dg, s0);
+                        store_split8(g.o[1].data + off, half * 8 + ch0 + ch, row, du, s1);
+                        store_split8(g.o[2].data + off, half * 8 + ch0 + ch, row, hh, s2);
                     }
                     });
                 }
             }
         }
+        if constexpr (SPL) cluster_sync();  // nobody leaves while its sums or maxima are read
     }
 }
 
-template <int CG, int NB, int EPI>
+template <int CG, int NB, int EPI, bool SPL = false>
 __global__ void __launch_bounds__(kXThreads, 1)
     split_mm_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mm,
                     const __grid_constant__ XArgs g) {
@@ -1007,10 +1088,13 @@ __global__ void __launch_bounds__(kXThreads, 1)
     uint64_t* drain = tempty + 2;
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain + 1);
     uint32_t* red = tmem_holder + 1;                       // three sets of four block maxima
-    int* last_flag = reinterpret_cast<int*>(red + 12);
+    // the cluster barriers that the epilogue warps of an SPL kernel meet at
+    constexpr int kSplitSyncs = !SPL ? 0 : EPI == kXF32 ? 2 : 3;
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const uint32_t rank = CG == 1 ? 0u : cluster_ctarank();
+    // CTAs 2 p and 2 p + 1 of a cluster are a pair
+    const uint32_t rank = CG == 1 ? 0u : cluster_ctarank() & 1u;
+    const uint32_t leader = CG == 1 ? 0u : cluster_ctarank() & ~1u;
     const int first = static_cast<int>(blockIdx.x) / CG, step = static_cast<int>(gridDim.x) / CG;
 
     grid_dependents_go();
@@ -1047,10 +1131,13 @@ __global__ void __launch_bounds__(kXThreads, 1)
 
     if (warp == 0) {
         if (lane == 0)
-            x_producer<CG, NB, EPI>(g, &mk, &mm, stages, full, empty, rank, first, step);
+            x_producer<CG, NB, EPI>(g, &mk, &mm, stages, full, empty, rank, leader, first, step);
+        __syncwarp();
+#pragma unroll
+        for (int s = 0; s < kSplitSyncs; ++s) cluster_sync();
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
-            x_mma<CG, NB, EPI>(g, tmem, stages, full, empty, tfull, tempty, first, step);
+            x_mma<CG, NB, EPI>(g, tmem, stages, full, empty, tfull, tempty, leader, first, step);
             // every MMA issued above must finish before TMEM is released, also on an error exit
             if constexpr (CG == 1) {
                 mma_commit(drain);
@@ -1060,9 +1147,11 @@ __global__ void __launch_bounds__(kXThreads, 1)
             mbar_wait(drain, 0, 1u << 1);
         }
         __syncwarp();
+#pragma unroll
+        for (int s = 0; s < kSplitSyncs; ++s) cluster_sync();
     } else {
-        x_epilogue<CG, NB, EPI>(g, epi_smem, red, last_flag, tmem, tfull, tempty, rank, first,
-                                step);
+        x_epilogue<CG, NB, EPI, SPL>(g, stages, epi_smem, red, tmem, tfull, tempty, rank, leader,
+                                     first, step);
     }
     tc_fence_before();
     __syncthreads();

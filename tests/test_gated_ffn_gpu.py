@@ -87,7 +87,8 @@ def inputs(cuda, rows, d, f, seed=0):
 
 
 SIZES = [(1, 1, 1), (2, 3, 5), (1, 1024, 640), (3, 257, 1030), (7, 96, 2050), (8, 640, 4096),
-         (13, 500, 333), (16, 1028, 260), (17, 64, 96), (33, 65, 127), (64, 128, 256), (127, 129, 255),
+         (13, 500, 333), (16, 1028, 260), (17, 64, 96), (20, 700, 2304), (33, 65, 127), (90, 1500, 260),
+         (128, 516, 3000), (64, 128, 256), (127, 129, 255),
          (128, 256, 128), (200, 100, 300), (257, 384, 513), (300, 1003, 771), (1031, 520, 900)]
 
 
@@ -110,7 +111,7 @@ def test_forward_and_backward(cuda, shape, act):
     assert mf.device_status() == 0
 
 
-@pytest.mark.parametrize("rows", [1, 2, 4, 5, 16, 40])
+@pytest.mark.parametrize("rows", [1, 2, 4, 5, 16, 40, 128, 129])
 @pytest.mark.parametrize("d,f", [(64, 200), (129, 333), (1024, 516), (2, 1)])
 def test_weights_stored_outputs_first(cuda, rows, d, f):
     """transpose_w: the same block from [outputs, inputs] weights, gradients in their layout."""
