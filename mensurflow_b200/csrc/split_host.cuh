@@ -396,7 +396,6 @@ int run_gated_ffn(const mfk_gated_ffn_desc* d, float* y, int64_t ldy, float* sav
     g.nb = static_cast<int>((d->d + 127) / 128);
     g.m = static_cast<int>(d->rows);
     g.n = static_cast<int>(d->d);
-    g.alpha = 1.0f;
     g.out = y;
     g.ld = ldy;
     return x_product<mfk::kXF32>(ws, g, d->f, 0, 1);
@@ -418,7 +417,6 @@ int x_weight_grad(XWorkspace& ws, const XMat& a, const XMat& b, int64_t rows, in
     g.n = static_cast<int>(t ? rows : cols);
     g.mb = (g.m + 127) / 128;
     g.nb = (g.n + 127) / 128;
-    g.alpha = 1.0f;
     g.out = out;
     g.ld = t ? cs : rs;
     g.out_bs = out_bs;
@@ -512,7 +510,6 @@ int run_gated_ffn_backward(const mfk_gated_ffn_desc* d, const mfk_gated_ffn_grad
         g.nb = static_cast<int>((d->d + 127) / 128);
         g.m = static_cast<int>(d->rows);
         g.n = static_cast<int>(d->d);
-        g.alpha = 1.0f;
         g.out = o->dx;
         g.ld = o->ld_dx;
         rc = x_product<mfk::kXF32>(ws, g, d->f, d->f, 1);
@@ -591,7 +588,8 @@ int run_orthogonalize(const float* u, int64_t batch, int64_t rows, int64_t cols,
     XMat x0;
     if (!x_source(ws, list, &x0, u, rows, cols, rs, 1, batch, bs)) return MFK_ERR_UNSUPPORTED;
     XMat x1 = steps > 1 ? x_mat(ws, rows, cols, batch) : x0;
-    const XMat gram = x_mat(ws, k, k, batch), poly = x_mat(ws, k, k, batch);
+    const XMat gram = x_mat(ws, k, k, batch), quad = x_mat(ws, k, k, batch),
+               poly = x_mat(ws, k, k, batch);
     rc = x_allocate(ws, 0);
     if (rc != MFK_OK) return rc;
     const XMat* mats[1] = {&x0};
@@ -615,31 +613,35 @@ int run_orthogonalize(const float* u, int64_t batch, int64_t rows, int64_t cols,
     }
     XMat *x = &x0, *next = &x1;
     for (int step = 0; step < steps; ++step) {
-        {   // gram = x x^T (or x^T x): symmetric, lower blocks only
+        // With g the Gram matrix, a x + (b g + c g g) x = (a I + g (b I + c g)) x: the diagonals go
+        // into the factors as they are written, and no product reads a third matrix.
+        {   // gram = x x^T (or x^T x), quad = b I + c gram: symmetric, lower blocks only
             mfk::XArgs g{};
             g.a[0] = g.a[1] = g.b[0] = g.b[1] = x_operand(ws, *x, !tall);
             g.mb = g.nb = gram.rb;
             g.m = g.n = static_cast<int>(k);
             g.sym = 1;
-            g.alpha = 1.0f;
             g.o[0] = x_out(ws, gram);
+            g.o[1] = x_out(ws, quad);
+            g.second = 1;
+            g.scale1 = cc;
+            g.diag1 = cb;
             rc = x_product<mfk::kXSplit>(ws, g, depth, 0, batch);
             if (rc != MFK_OK) return rc;
         }
-        {   // poly = cb gram + cc gram gram
+        {   // poly = a I + gram quad: symmetric too
             mfk::XArgs g{};
-            g.a[0] = g.a[1] = g.b[0] = g.b[1] = x_operand(ws, gram, true, true);
+            g.a[0] = g.a[1] = x_operand(ws, gram, true, true);
+            g.b[0] = g.b[1] = x_operand(ws, quad, true, true);
             g.mb = g.nb = gram.rb;
             g.m = g.n = static_cast<int>(k);
             g.sym = 1;
-            g.alpha = cc;
-            g.beta = cb;
-            g.c = x_out(ws, gram);
             g.o[0] = x_out(ws, poly);
+            g.diag0 = ca;
             rc = x_product<mfk::kXSplit>(ws, g, k, 0, batch);
             if (rc != MFK_OK) return rc;
         }
-        // x = ca x + poly x (or x poly)
+        // x = poly x (or x poly)
         mfk::XArgs g{};
         if (tall) {
             g.a[0] = g.a[1] = x_operand(ws, *x, true);
@@ -652,9 +654,6 @@ int run_orthogonalize(const float* u, int64_t batch, int64_t rows, int64_t cols,
         g.nb = x->cb;
         g.m = static_cast<int>(rows);
         g.n = static_cast<int>(cols);
-        g.alpha = 1.0f;
-        g.beta = ca;
-        g.c = x_out(ws, *x);
         if (step + 1 < steps) {
             g.o[0] = x_out(ws, *next);
             rc = x_product<mfk::kXSplit>(ws, g, k, 0, batch);

@@ -41,7 +41,7 @@ constexpr int kXBlockLines = 32;
 constexpr int kXThreads = 320;             // TMA warp, MMA warp, eight epilogue warps
 constexpr int kXEpiWarp0 = 2;
 constexpr int kXEpiThreads = 256;
-constexpr int kXBoxFloats = 32 * 33;       // 32 x 32, rows one float apart from 32: no conflicts
+constexpr int kXBoxFloats = 32 * 32;
 
 enum XEpi : int { kXF32 = 0, kXSplit = 1, kXGated = 2, kXGatedBwd = 3 };
 
@@ -69,8 +69,9 @@ struct XArgs {
     int m, n;              // output entries
     int tiles_m, tiles_n, splits, units, sym;
     int tiles;             // per matrix
-    float alpha, beta;     // acc * alpha + C * beta
-    XOut c;                // C as a split matrix (beta != 0)
+    // split output: o[0] = acc + diag0 I, and with `second` o[1] = scale1 acc + diag1 I
+    int second;
+    float diag0, scale1, diag1;
     float* out;            // fp32 output, row stride ld, batch stride out_bs
     long long ld, out_bs;
     XOut o[3];             // split outputs: result / h; dgate, dup, h
@@ -700,18 +701,40 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
         const XUnit w = x_unit(g, u);
         const int i = w.tm * CG + static_cast<int>(rank);
         const int i_in = min(i, g.mb - 1);
+        // this CTA's groups of eight columns: ng of them from ch0
+        const int ch0 = SPL ? 8 * w.s / g.splits : 0;
+        const int ng = SPL ? 8 * (w.s + 1) / g.splits - ch0 : 8;
+        // Backward: gate and up come eight columns (a turn) at a time through two slots of the
+        // warp's box, each lane copying what it reads itself, two turns ahead; the first two turns
+        // while the product is still computed, and the rest of the tile into L2 by then.
+        const int turns = EPI == kXGatedBwd && i < g.mb ? min(NB, g.nb - w.tn * NB) * ng : 0;
+        auto fetch = [&](int turn) {
+            if (turn < turns) {
+                const int b = SPL ? turn / ng : turn >> 3, ch = turn - b * ng;
+                const long long at =
+                    ((static_cast<long long>(i * g.o[0].ldb + w.tn * NB + b) * 2 + half) * 64 +
+                     (ch0 + ch) * 8) * kXBlk + row * 4;
+                const uint32_t dst = smem_u32(box) + (turn & 1) * 2048 + lane * 16;
+                cp_async_16(dst, g.gate + at);
+                cp_async_16(dst + 512, g.gate + at + 4 * kXBlk);
+                cp_async_16(dst + 1024, g.up + at);
+                cp_async_16(dst + 1536, g.up + at + 4 * kXBlk);
+            }
+            cp_async_commit();
+        };
         if constexpr (EPI == kXGatedBwd) {
-            // the tile's gate and up into L2 while its product is computed
             for (int b = 0; b < NB; ++b) {
                 const int jb = w.tn * NB + b;
                 if (i < g.mb && jb < g.nb && w.s == 0) {
-                    const long long at = (static_cast<long long>(i) * g.o[0].ldb + jb) * 16384;
+                    const long long at = static_cast<long long>(i * g.o[0].ldb + jb) * 16384;
                     for (int x = et * 32; x < 16384; x += kXEpiThreads * 32) {
                         prefetch_l2(g.gate + at + x);
                         prefetch_l2(g.up + at + x);
                     }
                 }
             }
+            fetch(0);
+            fetch(1);
         }
         float acc[NB * 64];
 #pragma unroll
@@ -769,10 +792,7 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
                 tphase ^= 1u;
             }
         }
-        // this CTA's groups of eight columns: ng of them from ch0, at the front of acc
-        const int ch0 = SPL ? 8 * w.s / g.splits : 0;
-        const int ng = SPL ? 8 * (w.s + 1) / g.splits - ch0 : 8;
-        if constexpr (SPL) {
+        if constexpr (SPL) {  // (from here on at the front of acc)
             float4* mine = reinterpret_cast<float4*>(stages) + et;
 #pragma unroll
             for (int j = 0; j < NB * 16; ++j)
@@ -802,43 +822,6 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
         }
         const bool row_block = i < g.mb;
 
-        if constexpr (EPI == kXF32 || EPI == kXSplit) {
-            // value = alpha acc + beta C
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const int jb = w.tn * NB + b;
-                if (g.beta != 0.0f && row_block && jb < g.nb) {
-                    const int blk = w.z * g.c.bstride + i * g.c.ldb + jb;
-                    const float f = g.c.inv[blk] * g.beta;
-                    const uint8_t* p = g.c.data + static_cast<long long>(blk) * kXBlockBytes +
-                                       (half * 8 + ch0) * kXLineBytes + row * 16;
-#pragma unroll
-                    for (int ch = 0; ch < 8; ++ch) {
-                        if (SPL && ch >= ng) break;
-                        const uint4 hq = *reinterpret_cast<const uint4*>(p + ch * kXLineBytes);
-                        const uint4 lq = *reinterpret_cast<const uint4*>(p + ch * kXLineBytes +
-                                                                         kXBlockBytes / 2);
-                        const uint32_t hw[4] = {hq.x, hq.y, hq.z, hq.w};
-                        const uint32_t lw[4] = {lq.x, lq.y, lq.z, lq.w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float2 hf =
-                                __half22float2(*reinterpret_cast<const __half2*>(&hw[e]));
-                            const float2 lf =
-                                __half22float2(*reinterpret_cast<const __half2*>(&lw[e]));
-                            float& a0 = acc[b * 64 + ch * 8 + e * 2];
-                            float& a1 = acc[b * 64 + ch * 8 + e * 2 + 1];
-                            a0 = fmaf(hf.x + lf.x, f, a0 * g.alpha);
-                            a1 = fmaf(hf.y + lf.y, f, a1 * g.alpha);
-                        }
-                    }
-                } else if (g.alpha != 1.0f) {
-#pragma unroll
-                    for (int j = 0; j < 64; ++j) acc[b * 64 + j] *= g.alpha;
-                }
-            }
-        }
-
         if constexpr (EPI == kXF32 && SPL) {
             const int grow = i * kXBlk + row;
 #pragma unroll
@@ -863,27 +846,45 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
                 }
             }
         } else if constexpr (EPI == kXF32) {
-            // through a 32 x 32 box, so that a warp writes 32 consecutive columns of one row at a
-            // time, whatever the row stride
+            // through a 32 x 32 box (16-byte column group c of row r at c ^ (r % 8): no bank
+            // conflicts either way), so that eight lanes write 128 bytes of a row
+            const bool wide = ((reinterpret_cast<uintptr_t>(g.out) & 15u) == 0) &&
+                              (g.ld & 3) == 0 && (g.out_bs & 3) == 0;
+            const uint32_t box0 = smem_u32(box);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    const int col = (w.tn * NB + b) * kXBlk + half * 64 + t * 32 + lane;
-                    const int row0 = i * kXBlk + q * 32;
                     __syncwarp();
 #pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        box[lane * 33 + j] = acc[b * 64 + t * 32 + j];
+                    for (int c = 0; c < 8; ++c) {
+                        const float* v = acc + b * 64 + t * 32 + c * 4;
+                        st_shared_v4(box0 + lane * 128 + ((c ^ (lane & 7)) << 4), v[0], v[1], v[2],
+                                     v[3]);
+                    }
                     __syncwarp();
+                    const int col = (w.tn * NB + b) * kXBlk + half * 64 + t * 32 + (lane & 7) * 4;
+                    const int row0 = i * kXBlk + q * 32 + (lane >> 3);
                     if (row_block && col < g.n) {
-                        float* dst = g.out + w.z * g.out_bs +
-                                     static_cast<long long>(row0) * g.ld + col;
-                        const int rows = min(32, g.m - row0);
-#pragma unroll 8
-                        for (int r = 0; r < rows; ++r) {
-                            *dst = box[r * 33 + lane];
-                            dst += g.ld;
+                        float* dst = g.out + w.z * g.out_bs + static_cast<long long>(row0) * g.ld +
+                                     col;
+                        const long long step = 4 * g.ld;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int r = e * 4 + (lane >> 3);
+                            const float4 v =
+                                ld_shared_v4(box0 + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+                            if (row0 + e * 4 < g.m) {
+                                if (wide && col + 4 <= g.n) {
+                                    *reinterpret_cast<float4*>(dst) = v;
+                                } else {
+                                    dst[0] = v.x;
+                                    if (col + 1 < g.n) dst[1] = v.y;
+                                    if (col + 2 < g.n) dst[2] = v.z;
+                                    if (col + 3 < g.n) dst[3] = v.w;
+                                }
+                            }
+                            dst += step;
                         }
                     }
                 }
@@ -892,8 +893,15 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
 
         if constexpr (EPI == kXSplit) {
             uint32_t* slot = red + parity * 4;
+            // this thread's column, of those at the front of acc, on a diagonal block's diagonal
+            const int diag_at = row - half * 64 - ch0 * 8;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
+                if (g.diag0 != 0.0f && i == w.tn * NB + b) {
+#pragma unroll
+                    for (int j = 0; j < 64; ++j)
+                        if (j == diag_at && j < ng * 8) acc[b * 64 + j] += g.diag0;
+                }
                 x_max_into(slot + b, largest<64>(acc + b * 64));
             }
             parity = parity == 2 ? 0 : parity + 1;
@@ -913,15 +921,35 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
             for (int b = 0; b < NB; ++b) {
                 const int jb = w.tn * NB + b;
                 if (row_block && jb < g.nb) {
-                    const int blk = w.z * g.o[0].bstride + i * g.o[0].ldb + jb;
                     float s, inv;
-                    split_scale(__uint_as_float(top_of[b]), s, inv);
+                    const float top = __uint_as_float(top_of[b]);
+                    const int blk = w.z * g.o[0].bstride + i * g.o[0].ldb + jb;
+                    split_scale(top, s, inv);
                     if (et == 0 && w.s == 0) g.o[0].inv[blk] = inv;
                     uint8_t* dst = g.o[0].data + static_cast<long long>(blk) * kXBlockBytes;
 #pragma unroll
                     for (int ch = 0; ch < 8; ++ch)
                         if (ch < ng)
                             store_split8(dst, half * 8 + ch0 + ch, row, acc + b * 64 + ch * 8, s);
+                    if (g.second) {
+                        // its scale from a bound: no second maximum
+                        const int blk1 = w.z * g.o[1].bstride + i * g.o[1].ldb + jb;
+                        split_scale(fminf(fmaf(fabsf(g.scale1), top, fabsf(g.diag1)),
+                                          3.402823466e38f), s, inv);
+                        if (et == 0 && w.s == 0) g.o[1].inv[blk1] = inv;
+                        uint8_t* dst1 = g.o[1].data + static_cast<long long>(blk1) * kXBlockBytes;
+#pragma unroll
+                        for (int ch = 0; ch < 8; ++ch) {
+                            if (ch < ng) {
+                                float v[8];
+#pragma unroll
+                                for (int e = 0; e < 8; ++e)
+                                    v[e] = fmaf(acc[b * 64 + ch * 8 + e], g.scale1,
+                                                i == jb && ch * 8 + e == diag_at ? g.diag1 : 0.0f);
+                                store_split8(dst1, half * 8 + ch0 + ch, row, v, s);
+                            }
+                        }
+                    }
                 }
             }
         }
@@ -1024,33 +1052,20 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
                         g.o[1].inv[blk] = i1;
                         g.o[2].inv[blk] = i2;
                     }
-                    const long long at =
-                        ((static_cast<long long>(blk) * 2 + half) * 64 + ch0 * 8) * kXBlk +
-                        row * 4;
                     const long long off = static_cast<long long>(blk) * kXBlockBytes;
 with_act(g.act, [&](auto kind) {
-                    float4 gv[2], uv[2];  // eight columns, loaded one turn ahead
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        gv[e] = *reinterpret_cast<const float4*>(g.gate + at + e * 4 * kXBlk);
-                        uv[e] = *reinterpret_cast<const float4*>(g.up + at + e * 4 * kXBlk);
-                    }
 #pragma unroll
                     for (int ch = 0; ch < 8; ++ch) {
                         if (SPL && ch >= ng) break;
                         float dg[8], du[8], hh[8];
-                        const float gs[8] = {gv[0].x, gv[0].y, gv[0].z, gv[0].w,
-                                             gv[1].x, gv[1].y, gv[1].z, gv[1].w};
-                        const float us[8] = {uv[0].x, uv[0].y, uv[0].z, uv[0].w,
-                                             uv[1].x, uv[1].y, uv[1].z, uv[1].w};
-                        if (ch + 1 < ng) {
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const long long x = at + (ch * 8 + 8 + e * 4) * kXBlk;
-                                gv[e] = *reinterpret_cast<const float4*>(g.gate + x);
-                                uv[e] = *reinterpret_cast<const float4*>(g.up + x);
-                            }
-                        }
+                        const int turn = b * ng + ch;
+                        const uint32_t src = smem_u32(box) + (turn & 1) * 2048 + lane * 16;
+                        cp_async_wait<1>();
+                        const float4 g0 = ld_shared_v4(src), g1 = ld_shared_v4(src + 512);
+                        const float4 u0 = ld_shared_v4(src + 1024), u1 = ld_shared_v4(src + 1536);
+                        fetch(turn + 2);
+                        const float gs[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
+                        const float us[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
 #pragma unroll
                         for (int x = 0; x < 8; ++x) {
                             const float dh = acc[b * 64 + ch * 8 + x];
@@ -1067,6 +1082,7 @@ with_act(g.act, [&](auto kind) {
                 }
             }
         }
+        if constexpr (EPI == kXGatedBwd) cp_async_wait<0>();
         if constexpr (SPL) cluster_sync();  // nobody leaves while its sums or maxima are read
     }
 }
