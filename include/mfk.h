@@ -341,15 +341,17 @@ int mfk_copy_peer(void* dst, int32_t dst_device, const void* src, int32_t src_de
 /* The gated feed-forward block and its backward pass, in fp32:
  *     gate = x w_gate, up = x w_up, h = act(gate) * up, y = h w_down.
  * x is rows x d, w_gate and w_up d x f, w_down f x d; element (i, j) of a matrix at
- * p[i*rs + j*cs], and of each matrix's two strides one must be 1 (MFK_ERR_UNSUPPORTED otherwise;
- * weights stored [outputs, inputs] have rs = 1). w_gate and w_up must lie the same way round.
- * activation is any mfk_activation. No counterpart in the reference, which composes such blocks
- * from gemm and elementwise calls; like mfk_gemm_f32's 3xTF32 form the products are
- * fp32-faithful: each matrix is split into fp16 (hi, lo) pairs under one power-of-two scale per
- * 128 x 128 block, three products are summed, and sums are held in fp32 over any depth. An entry
- * keeps 22 bits or more while it is within 2^-17 of the largest entry of its block, and an
- * absolute error of 2^-39 of that entry below. A non-finite operand entry makes the results that
- * depend on it non-finite (an infinity may come out as NaN).
+ * p[i*rs + j*cs]. x_cs must be 1; of each other matrix's two strides one must be 1
+ * (MFK_ERR_UNSUPPORTED otherwise; weights stored [outputs, inputs] have rs = 1). w_gate and w_up must
+ * lie the same way round. activation is any mfk_activation. No counterpart in the reference, which
+ * composes such blocks from gemm and elementwise calls; like mfk_gemm_f32's 3xTF32 form the
+ * products are fp32-faithful: each matrix is split into fp16 (hi, lo) pairs under power-of-two
+ * scales, three products are summed, and sums are held in fp32 over any depth. The rows of x and
+ * of h have a scale each per 128 columns, so no row of y depends on another; the weights, and in
+ * the backward pass every matrix, have one per 128 x 128 block. Under one scale an entry keeps 22
+ * bits or more while it is within 2^-17 of the largest, and an absolute error of 2^-39 of that one
+ * below. A non-finite operand entry makes the results that depend on it non-finite (an infinity may
+ * come out as NaN). Up to 16 rows without `saved` are plain fp32 sums.
  *
  * mfk_gated_ffn_f32: y has row stride ldy >= d. saved (optional, 16-byte aligned,
  * mfk_gated_ffn_saved_floats(rows, f) floats of device memory) receives gate and up for the
@@ -361,7 +363,9 @@ int mfk_copy_peer(void* dst, int32_t dst_device, const void* src, int32_t src_de
  * saved: what the forward call with the same x, w_gate, w_up left, or NULL (recomputed). dx may be
  * NULL, and the three weight gradients may be NULL together. dw_gate and dw_up share their
  * strides; of each output's strides one must be 1. The gradients are written, not added to, and
- * must not overlap the inputs or each other. rows = 0 gives zero weight gradients.
+ * must not overlap the inputs or each other. rows = 0 gives zero weight gradients. A row whose
+ * grad is all zero (padding) adds nothing to the weight gradients, whatever finite or non-finite
+ * values x has there.
  *
  * Both take their workspace from the stream-ordered allocator. */
 typedef struct mfk_gated_ffn_desc {
@@ -413,12 +417,12 @@ int mfk_orthogonalize_f32(const float* update, int64_t batch, int64_t rows, int6
  * id_bytes 4 or 8 (signed). No counterpart in the reference.
  *
  * mfk_embedding_f32: out[i] = scale * table[ids[i]] for the n ids; table is rows x d with row
- * stride ld >= d, out n x d with row stride ld_out >= d. An id outside [0, rows) gives a row of
+ * stride ld (any, 0 for one row seen many times), out n x d with row stride ld_out >= d. An id outside [0, rows) gives a row of
  * zeros and sets MFK_DEVERR_INDEX in the device error word.
  *
  * mfk_embedding_grad_f32: out[v] = scale * (sum of grad[i] over the i with ids[i] == v) for every
  * v of [0, rows): a dense gradient, rows that no id names are zeros. grad is n x d with row stride
- * ld_grad >= d, out rows x d with row stride ld >= d (written, not added to). Tokens whose id is
+ * ld_grad (any, 0 broadcasts), out rows x d with row stride ld >= d (written, not added to). Tokens whose id is
  * `padding` take no part (-1: none is left out); an id outside [0, rows) that is not `padding`
  * takes no part either and sets MFK_DEVERR_INDEX. The sums are fp32, in an order that depends on
  * the ids and sizes alone, so repeated calls give the same bits. The workspace (16 bytes per

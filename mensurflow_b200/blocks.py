@@ -116,6 +116,8 @@ def _gated_args(op, x, w_gate, w_up, w_down, activation, transpose_w):
     for s in x.shape[:-1]:
         rows *= s
     x2 = _rows_of(x, rows, d)
+    if _lies(x2):  # a scale for every row: rows have to be contiguous
+        x2 = contiguous(x2)
     gate, up, down = _unit(gate), _unit(up), _unit(down)
     if _lies(gate) != _lies(up):  # the two projections share a tile: one way round
         gate, up = contiguous(gate), contiguous(up)
@@ -155,10 +157,12 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     With ``save`` the result is (y, saved): ``saved`` spares ``gated_ffn_backward`` the two
     projections at the price of 8 bytes per row and feature.
 
-    The products are fp32-faithful (fp16 pairs under one power-of-two scale per 128 x 128 block,
-    sums in fp32), whatever ``set_default_precision`` says; an entry more than 2^17 below the
-    largest of its block keeps an absolute error of 2^-39 of that largest one. Non-finite inputs
-    give non-finite results, though an infinity may come out as NaN."""
+    The products are fp32-faithful (fp16 pairs under power-of-two scales, sums in fp32), whatever
+    ``set_default_precision`` says. Rows of x and of the hidden values have scales of their own, so
+    no row of the result depends on another; a weight more than 2^17 below the largest of its
+    128 x 128 block keeps an absolute error of 2^-39 of that one. Non-finite inputs give non-finite
+    results, though an infinity may come out as NaN. Up to 16 rows, without ``save``, run as plain
+    fp32 sums at the speed the weights are read."""
     desc, keep = _gated_args("gated_ffn", x, w_gate, w_up, w_down, activation, transpose_w)
     rows, d, f = desc.rows, desc.d, desc.f
     so = _lib.lib()
@@ -178,7 +182,9 @@ def gated_ffn_backward(grad: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor
     """(dx, dw_gate, dw_up, dw_down) of ``gated_ffn`` for grad = dL/dy, with the forward call's
     arguments; dx has x's shape and the weights' gradients have the weights' own layouts.
     ``saved`` from the forward call with the same x and weights; without it the two projections
-    are computed again. What is not needed is None."""
+    are computed again. What is not needed is None. A row whose gradient is all zero (padding) adds
+    nothing to the weights' gradients, whatever x holds there. Arithmetic as in ``gated_ffn``, with
+    one scale per 128 x 128 block."""
     op = "gated_ffn_backward"
     desc, keep = _gated_args(op, x, w_gate, w_up, w_down, activation, transpose_w)
     _require(grad, op, "grad")
@@ -277,7 +283,7 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0) -> tor
     out = table.new_empty(ids.shape + (d,))
     if n and d:
         _run(table.device, op, _lib.lib().mfk_embedding_f32, t.data_ptr(), rows, d,
-             max(t.stride(0), d), index.data_ptr(), index.element_size(), n, float(scale),
+             t.stride(0) if rows > 1 else d, index.data_ptr(), index.element_size(), n, float(scale),
              out.data_ptr(), d)
     return out
 

@@ -80,7 +80,7 @@ int run_embedding_grad(const float* grad, int64_t n, int64_t d, int64_t ld_grad,
     if (rc != MFK_OK) return rc;
     if (rows == 0 || d == 0) return MFK_OK;
     if (out == nullptr || ld < d) return MFK_ERR_INVALID_ARGUMENT;
-    if (n > 0 && (grad == nullptr || ids == nullptr || (ld_grad < d && n > 1)))
+    if (n > 0 && (grad == nullptr || ids == nullptr || ld_grad < 0))
         return MFK_ERR_INVALID_ARGUMENT;
     int dev = 0;
     DeviceInfo* info = nullptr;
@@ -182,7 +182,7 @@ int mfk_embedding_f32(const float* table, int64_t rows, int64_t d, int64_t ld, c
     if (rc != MFK_OK) return rc;
     if (n == 0 || d == 0) return MFK_OK;
     if (rows == 0 || table == nullptr || ids == nullptr || out == nullptr || ld_out < d ||
-        (ld < d && rows > 1))
+        ld < 0)
         return MFK_ERR_INVALID_ARGUMENT;
     int dev = 0;
     DeviceInfo* info = nullptr;

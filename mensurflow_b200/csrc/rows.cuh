@@ -37,12 +37,6 @@ struct RowsArgs {
     int wait;                // x comes from the launch before
 };
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-    return v;
-}
-
 // 4, 8 or 16 bytes, global -> shared, in the thread's own copy groups.
 template <int BYTES>
 __device__ __forceinline__ void rows_copy(float* dst, const float* src) {

@@ -18,6 +18,8 @@ struct XMat {
     int64_t rows = 0, cols = 0, batch = 1;  // as stored
     int rb = 0, cb = 0;                     // blocks
     int64_t first = 0;                      // index of its first block in the workspace
+    int64_t inv = 0;                        // and of its first 1/s
+    bool by_row = false;                    // a scale for every row of a block
     bool transposed = false;                // stored as the logical matrix's transpose
 
     int64_t blocks() const { return static_cast<int64_t>(rb) * cb; }
@@ -32,7 +34,7 @@ struct XWorkspace {
     float* inv = nullptr;
     double* sumsq = nullptr;
     float* extra = nullptr;
-    int64_t total_blocks = 0;
+    int64_t total_blocks = 0, total_inv = 0;
     CUtensorMap mk, mm;
     int dev = 0;
     DeviceInfo* info = nullptr;
@@ -45,15 +47,18 @@ struct XWorkspace {
     }
 };
 
-XMat x_mat(XWorkspace& ws, int64_t rows, int64_t cols, int64_t batch = 1) {
+XMat x_mat(XWorkspace& ws, int64_t rows, int64_t cols, int64_t batch = 1, bool by_row = false) {
     XMat m;
+    m.by_row = by_row;
     m.rows = rows;
     m.cols = cols;
     m.batch = batch;
     m.rb = static_cast<int>((rows + mfk::kXBlk - 1) / mfk::kXBlk);
     m.cb = static_cast<int>((cols + mfk::kXBlk - 1) / mfk::kXBlk);
     m.first = ws.total_blocks;
+    m.inv = ws.total_inv;
     ws.total_blocks += m.blocks() * batch;
+    ws.total_inv += m.blocks() * batch * (by_row ? mfk::kXBlk : 1);
     return m;
 }
 
@@ -71,7 +76,7 @@ bool x_orientation(int64_t rows, int64_t cols, int64_t rs, int64_t cs, bool* tra
 int x_allocate(XWorkspace& ws, size_t extra_floats) {
     if (ws.total_blocks > (int64_t(1) << 25)) return MFK_ERR_UNSUPPORTED;  // 2 TB of blocks
     const size_t block_bytes = static_cast<size_t>(ws.total_blocks) * mfk::kXBlockBytes;
-    const size_t inv_bytes = (static_cast<size_t>(ws.total_blocks) * 4 + 255) / 256 * 256;
+    const size_t inv_bytes = (static_cast<size_t>(ws.total_inv) * 4 + 255) / 256 * 256;
     const size_t sum_bytes = (static_cast<size_t>(ws.total_blocks) * 8 + 255) / 256 * 256;
     const size_t total = block_bytes + inv_bytes + sum_bytes + extra_floats * 4 + 1024;
     MFK_CUDA(cudaMallocAsync(reinterpret_cast<void**>(&ws.base), total, ws.stream));
@@ -104,10 +109,11 @@ int x_allocate(XWorkspace& ws, size_t extra_floats) {
 // Adds logical matrix (rows x cols at p, strides rs, cs; batch matrices bs apart) to the split
 // pass and to the workspace. False: neither stride is 1.
 bool x_source(XWorkspace& ws, mfk::XSources& list, XMat* out, const float* p, int64_t rows,
-              int64_t cols, int64_t rs, int64_t cs, int64_t batch = 1, int64_t bs = 0) {
+              int64_t cols, int64_t rs, int64_t cs, int64_t batch = 1, int64_t bs = 0,
+              bool by_row = false) {
     bool t = false;
-    if (!x_orientation(rows, cols, rs, cs, &t)) return false;
-    *out = x_mat(ws, t ? cols : rows, t ? rows : cols, batch);
+    if (!x_orientation(rows, cols, rs, cs, &t) || (by_row && t)) return false;
+    *out = x_mat(ws, t ? cols : rows, t ? rows : cols, batch, by_row);
     out->transposed = t;
     mfk::XSource& s = list.s[list.count++];
     s = mfk::XSource{};
@@ -119,6 +125,7 @@ bool x_source(XWorkspace& ws, mfk::XSources& list, XMat* out, const float* p, in
     s.batch = static_cast<int>(batch);
     s.rb = out->rb;
     s.cb = out->cb;
+    s.by_row = by_row ? 1 : 0;
     s.vec = aligned16(p) && (s.rs % 4 == 0 || out->rows <= 1) && s.bs % 4 == 0;
     return true;
 }
@@ -129,7 +136,7 @@ int x_split(XWorkspace& ws, mfk::XSources& list, const XMat* const* mats, bool s
         mfk::XSource& s = list.s[i];
         s.first = static_cast<int>(at);
         s.data = ws.blocks + mats[i]->first * mfk::kXBlockBytes;
-        s.inv = ws.inv + mats[i]->first;
+        s.inv = ws.inv + mats[i]->inv;
         s.sumsq = sums ? ws.sumsq + mats[i]->first : nullptr;
         at += mats[i]->blocks() * mats[i]->batch;
     }
@@ -148,14 +155,15 @@ mfk::XOperand x_operand(const XWorkspace& ws, const XMat& m, bool over_columns, 
     o.bstride = m.batch > 1 ? static_cast<int>(m.blocks()) : 0;
     o.flip = over_columns == m.transposed ? 1 : 0;
     o.sym = sym ? 1 : 0;
-    o.inv = ws.inv + m.first;
+    o.by_row = m.by_row ? 1 : 0;
+    o.inv = ws.inv + m.inv;
     return o;
 }
 
 mfk::XOut x_out(const XWorkspace& ws, const XMat& m) {
     mfk::XOut o{};
     o.data = ws.blocks + m.first * mfk::kXBlockBytes;
-    o.inv = ws.inv + m.first;
+    o.inv = ws.inv + m.inv;
     o.ldb = m.cb;
     o.bstride = m.batch > 1 ? static_cast<int>(m.blocks()) : 0;
     return o;
@@ -327,7 +335,7 @@ int check_gated(const mfk_gated_ffn_desc* d) {
 
 int64_t gated_saved_floats(int64_t rows, int64_t f) {
     const int64_t blocks = ((rows + 127) / 128) * ((f + 127) / 128);
-    return blocks * (2 * 128 * 128 + 2);
+    return blocks * (2 * 128 * 128 + 4 * 128);
 }
 
 // gate and up (and h, when `h` is given) of x: one product whose tiles hold both projections.
@@ -375,13 +383,13 @@ int run_gated_ffn(const mfk_gated_ffn_desc* d, float* y, int64_t ldy, float* sav
         return run_gated_rows(d, y, ldy, ws.info, ws.dev, stream);
     mfk::XSources list{};
     XMat x, wg, wu, wd;
-    if (!x_source(ws, list, &x, d->x, d->rows, d->d, d->x_rs, d->x_cs) ||
+    if (!x_source(ws, list, &x, d->x, d->rows, d->d, d->x_rs, d->x_cs, 1, 0, true) ||
         !x_source(ws, list, &wg, d->w_gate, d->d, d->f, d->w_gate_rs, d->w_gate_cs) ||
         !x_source(ws, list, &wu, d->w_up, d->d, d->f, d->w_up_rs, d->w_up_cs) ||
         !x_source(ws, list, &wd, d->w_down, d->f, d->d, d->w_down_rs, d->w_down_cs))
         return MFK_ERR_UNSUPPORTED;
     if (wg.transposed != wu.transposed) return MFK_ERR_UNSUPPORTED;
-    const XMat h = x_mat(ws, d->rows, d->f);
+    const XMat h = x_mat(ws, d->rows, d->f, 1, true);
     rc = x_allocate(ws, 0);
     if (rc != MFK_OK) return rc;
     const XMat* mats[4] = {&x, &wg, &wu, &wd};
@@ -457,26 +465,38 @@ int run_gated_ffn_backward(const mfk_gated_ffn_desc* d, const mfk_gated_ffn_grad
         return rc;
     }
     mfk::XSources list{};
-    XMat x, wg, wu, wd, dy;
+    // x twice where the projections are computed again: by rows for them, in blocks for the sums
+    // over rows.
+    XMat x, wg, wu, wd, dy, x_rows;
     if (!x_source(ws, list, &x, d->x, d->rows, d->d, d->x_rs, d->x_cs) ||
         !x_source(ws, list, &wg, d->w_gate, d->d, d->f, d->w_gate_rs, d->w_gate_cs) ||
         !x_source(ws, list, &wu, d->w_up, d->d, d->f, d->w_up_rs, d->w_up_cs) ||
         !x_source(ws, list, &wd, d->w_down, d->f, d->d, d->w_down_rs, d->w_down_cs) ||
-        !x_source(ws, list, &dy, o->grad, d->rows, d->d, o->grad_rs, o->grad_cs))
+        !x_source(ws, list, &dy, o->grad, d->rows, d->d, o->grad_rs, o->grad_cs) || x.transposed)
         return MFK_ERR_UNSUPPORTED;
     if (wg.transposed != wu.transposed) return MFK_ERR_UNSUPPORTED;
+    if (saved == nullptr &&
+        !x_source(ws, list, &x_rows, d->x, d->rows, d->d, d->x_rs, d->x_cs, 1, 0, true))
+        return MFK_ERR_UNSUPPORTED;
     const XMat dg = x_mat(ws, d->rows, d->f);
     const XMat du = x_mat(ws, d->rows, d->f);  // directly behind dg: a batch of two
     const XMat h = x_mat(ws, d->rows, d->f);
     const int64_t saved_floats = gated_saved_floats(d->rows, d->f);
-    rc = x_allocate(ws, saved == nullptr ? static_cast<size_t>(saved_floats) : 0);
+    const size_t again = saved == nullptr ? static_cast<size_t>(saved_floats) : 0;
+    rc = x_allocate(ws, again + static_cast<size_t>(d->rows));
     if (rc != MFK_OK) return rc;
-    const XMat* mats[5] = {&x, &wg, &wu, &wd, &dy};
+    int* live = reinterpret_cast<int*>(ws.extra + again);
+    mfk::live_rows_kernel<<<static_cast<unsigned>((d->rows + 7) / 8), 256, 0, stream>>>(
+        o->grad, o->grad_rs, o->grad_cs, static_cast<int>(d->rows), static_cast<int>(d->d), live);
+    g_launches.fetch_add(1);
+    MFK_CUDA(cudaGetLastError());
+    list.s[0].live = live;
+    const XMat* mats[6] = {&x, &wg, &wu, &wd, &dy, &x_rows};
     rc = x_split(ws, list, mats, false);
     if (rc != MFK_OK) return rc;
     const float* pre = saved;
     if (pre == nullptr) {
-        rc = gated_forward(ws, d, x, wg, wu, nullptr, ws.extra);
+        rc = gated_forward(ws, d, x_rows, wg, wu, nullptr, ws.extra);
         if (rc != MFK_OK) return rc;
         pre = ws.extra;
     }
@@ -494,6 +514,7 @@ int run_gated_ffn_backward(const mfk_gated_ffn_desc* d, const mfk_gated_ffn_grad
         g.gate = p;
         g.up = p + blocks * 128 * 128;
         g.gmax = p + blocks * 2 * 128 * 128;
+        g.live = live;
         g.o[0] = x_out(ws, dg);
         g.o[1] = x_out(ws, du);
         g.o[2] = x_out(ws, h);
@@ -608,7 +629,7 @@ int run_orthogonalize(const float* u, int64_t batch, int64_t rows, int64_t cols,
         cfg.numAttrs = 1;
         MFK_CUDA(cudaLaunchKernelEx(&cfg, mfk::split_normalize_kernel,
                                     static_cast<const double*>(ws.sumsq + x0.first),
-                                    ws.inv + x0.first, static_cast<int>(x0.blocks()), eps));
+                                    ws.inv + x0.inv, static_cast<int>(x0.blocks()), eps));
         g_launches.fetch_add(1);
     }
     XMat *x = &x0, *next = &x1;

@@ -5,7 +5,8 @@
 // block's largest magnitude into [2^14, 2^15), each entry x of the block is held as two halves,
 //     hi = fp16(s x),  lo = fp16(s x - hi),
 // so s x = hi + lo to 2^-23 of itself (and never worse than 2^-40 of the block's largest entry:
-// lo's spacing ends at 2^-24). A product of two such matrices takes three fp16 products,
+// lo's spacing ends at 2^-24). An operand whose rows are the result's rows may have one s per row
+// of a block instead (`by_row`): then no row's accuracy depends on another's size. A product of two such matrices takes three fp16 products,
 //     (s_a a)(s_b b) ~ lo hi + hi lo + hi hi,
 // summed in fp32; the term left out, lo lo, is below 2^-22 of the product. fp16 tensor products
 // run at twice the tf32 rate, so this is twice as fast as a tf32 three-way split of the same 22
@@ -52,7 +53,8 @@ struct XOperand {
     int bstride;      // blocks from one matrix of a batch to the next
     int flip;         // 0: contraction along the stored columns, 1: along the stored rows
     int sym;          // symmetric: only blocks (i, j) with i >= j are stored
-    const float* inv; // 1/s per block
+    int by_row;       // a scale for every row of a block
+    const float* inv; // 1/s per block, or per row of a block
 };
 
 struct XOut {
@@ -77,7 +79,8 @@ struct XArgs {
     XOut o[3];             // split outputs: result / h; dgate, dup, h
     float* gate;           // saved pre-activations in accumulator order (null: not saved)
     float* up;
-    float* gmax;           // largest |gate|, |up| per block
+    float* gmax;           // largest |gate| and |up| of 64 columns: per block [2][2 halves][128]
+    const int* live;       // backward: 0 for the rows whose gradient is all zero
     int act;
     int store_h;
 };
@@ -165,6 +168,12 @@ __device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
                  : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
                  : "r"(addr)
                  : "memory");
+    return v;
+}
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
     return v;
 }
 
@@ -257,9 +266,11 @@ struct XSource {
     uint8_t* data;
     float* inv;
     double* sumsq;         // per-block sum of squares, or null
+    const int* live;       // rows to leave out (0) as if they were zero, or null
+    int by_row;            // a scale for every row
 };
 
-constexpr int kXMaxSources = 5;
+constexpr int kXMaxSources = 6;
 struct XSources {
     XSource s[kXMaxSources];
     int count;
@@ -288,7 +299,7 @@ __global__ void __launch_bounds__(256) split_blocks_kernel(const __grid_constant
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
         const int row = bi * kXBlk + (warp * 2 + a) * 8 + r8;
-        const bool row_ok = row < t.rows;
+        const bool row_ok = row < t.rows && (t.live == nullptr || t.live[row] != 0);
         const float* p = base + static_cast<long long>(row_ok ? row : 0) * t.rs;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
@@ -342,7 +353,7 @@ __global__ void __launch_bounds__(256) split_blocks_kernel(const __grid_constant
     float s, inv;
     split_scale(__uint_as_float(all), s, inv);
     if (threadIdx.x == 0) {
-        t.inv[local] = inv;
+        if (!t.by_row) t.inv[local] = inv;
         if (t.sumsq != nullptr) {
             double total = 0.0;
 #pragma unroll
@@ -352,10 +363,35 @@ __global__ void __launch_bounds__(256) split_blocks_kernel(const __grid_constant
     }
     uint8_t* block = t.data + static_cast<long long>(local) * kXBlockBytes;
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
+    for (int a = 0; a < 2; ++a) {
+        const int row = (warp * 2 + a) * 8 + r8;
+        if (t.by_row) {  // a row's 128 columns lie in four lanes
+            float m = largest<32>(&v[a][0][0]);
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            split_scale(m, s, inv);
+            if (c4 == 0) t.inv[static_cast<long long>(local) * kXBlk + row] = inv;
+        }
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-            store_split8(block, b * 4 + c4, (warp * 2 + a) * 8 + r8, v[a][b], s);
+        for (int b = 0; b < 4; ++b) store_split8(block, b * 4 + c4, row, v[a][b], s);
+    }
+}
+
+// live[r] = whether row r of the rows x cols matrix has an entry other than zero: a warp per row,
+// which stops at the first 32 columns that have one.
+__global__ void __launch_bounds__(256)
+    live_rows_kernel(const float* __restrict__ p, long long rs, long long cs, int rows, int cols,
+                     int* __restrict__ live) {
+    grid_dependents_go();
+    const int lane = threadIdx.x & 31;
+    const int r = static_cast<int>((static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) >> 5);
+    if (r >= rows) return;
+    bool any = false;
+    for (int c = 0; c < cols && !any; c += 32) {
+        const bool mine = c + lane < cols && !(p[r * rs + (c + lane) * cs] == 0.0f);
+        any = __any_sync(0xffffffffu, mine);
+    }
+    if (lane == 0) live[r] = any ? 1 : 0;
 }
 
 // Divides matrix z of a batch by its Frobenius norm (+ eps) by scaling the blocks' 1/s: exact up
@@ -742,8 +778,10 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
         for (int c = w.c0; c < w.c1; ++c) {
             const int seg = EPI == kXF32 && c >= g.kc0 ? 1 : 0;
             const int k = seg ? c - g.kc0 : c;
-            const float ia =
-                g.a[seg].inv[x_block(g.a[seg], w.z, i_in, k, x_flip(g.a[seg], w.tm * CG, k))];
+            const int a_blk = x_block(g.a[seg], w.z, i_in, k, x_flip(g.a[seg], w.tm * CG, k));
+            const float ia = g.a[seg].by_row
+                                 ? g.a[seg].inv[static_cast<long long>(a_blk) * kXBlk + row]
+                                 : g.a[seg].inv[a_blk];
             float f1[NB], f2[NB];  // the two blocks' 1/s: multiplied together where that is safe
             bool safe = true;
 #pragma unroll
@@ -892,7 +930,7 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
         }
 
         if constexpr (EPI == kXSplit) {
-            uint32_t* slot = red + parity * 4;
+            uint32_t* slot = red + parity * 8;
             // this thread's column, of those at the front of acc, on a diagonal block's diagonal
             const int diag_at = row - half * 64 - ch0 * 8;
 #pragma unroll
@@ -905,7 +943,7 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
                 x_max_into(slot + b, largest<64>(acc + b * 64));
             }
             parity = parity == 2 ? 0 : parity + 1;
-            if (et < 4) red[parity * 4 + et] = 0u;
+            if (et < 8) red[parity * 8 + et] = 0u;
             epi_bar();
             uint32_t top_of[3] = {slot[0], slot[1], slot[2]};
             if constexpr (SPL) {
@@ -955,12 +993,14 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
         }
 
         if constexpr (EPI == kXGated) {
-            // acc: 64 gate columns, then the same 64 up columns
-            uint32_t* slot = red + parity * 4;
+            // acc: 64 gate columns, then the same 64 up columns. Row maxima of h, gate and up go
+            // through the (otherwise idle) boxes: two sets of [3][2 halves][128] take turns.
+            float* rowmax = reinterpret_cast<float*>(epi_smem) + (parity & 1) * (6 * kXBlk);
+            ++parity;
             const int blk = i_in * g.o[0].ldb + w.tn;
             if (g.gate != nullptr) {
-                x_max_into(slot + 1, largest<64>(acc));
-                x_max_into(slot + 2, largest<64>(acc + 64));
+                rowmax[(2 + half) * kXBlk + row] = largest<64>(acc);
+                rowmax[(4 + half) * kXBlk + row] = largest<64>(acc + 64);
             }
             const long long at =
                 ((static_cast<long long>(blk) * 2 + half) * 64 + ch0 * 8) * kXBlk + row * 4;
@@ -981,29 +1021,31 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
                         acc[e] = act_slope<decltype(kind)::value>(acc[e]).x * acc[64 + e];
                 }
             });
-            if (g.store_h) x_max_into(slot, largest<64>(acc));
-            parity = parity == 2 ? 0 : parity + 1;
-            if (et < 4) red[parity * 4 + et] = 0u;
+            if (g.store_h) rowmax[half * kXBlk + row] = largest<64>(acc);
             epi_bar();
-            uint32_t top_of[3] = {slot[0], slot[1], slot[2]};
+            float hm = fmaxf(rowmax[row], rowmax[kXBlk + row]);
+            float gm = rowmax[(2 + half) * kXBlk + row], um = rowmax[(4 + half) * kXBlk + row];
             if constexpr (SPL) {
                 cluster_sync();
                 for (int r = 0; r < g.splits; ++r) {
-                    const uint32_t at = mapa_shared(slot, r * CG + rank);
-#pragma unroll
-                    for (int e = 0; e < 3; ++e)
-                        top_of[e] = max(top_of[e], ld_cluster_u32(at + e * 4));
+                    const uint32_t from = mapa_shared(rowmax + row, r * CG + rank);
+                    hm = fmaxf(hm, fmaxf(ld_cluster_f32(from), ld_cluster_f32(from + kXBlk * 4)));
+                    gm = fmaxf(gm, ld_cluster_f32(from + (2 + half) * kXBlk * 4));
+                    um = fmaxf(um, ld_cluster_f32(from + (4 + half) * kXBlk * 4));
                 }
             }
             if (row_block) {
-                if (g.gate != nullptr && et == 0 && w.s == 0) {
-                    g.gmax[blk * 2] = __uint_as_float(top_of[1]);
-                    g.gmax[blk * 2 + 1] = __uint_as_float(top_of[2]);
+                if (g.gate != nullptr && w.s == 0) {
+                    float* to = g.gmax + static_cast<long long>(blk) * 4 * kXBlk + half * kXBlk +
+                                row;
+                    to[0] = gm;
+                    to[2 * kXBlk] = um;
                 }
                 if (g.store_h) {
                     float s, inv;
-                    split_scale(__uint_as_float(top_of[0]), s, inv);
-                    if (et == 0 && w.s == 0) g.o[0].inv[blk] = inv;
+                    split_scale(hm, s, inv);
+                    if (half == 0 && w.s == 0)
+                        g.o[0].inv[static_cast<long long>(blk) * kXBlk + row] = inv;
                     uint8_t* dst = g.o[0].data + static_cast<long long>(blk) * kXBlockBytes;
 #pragma unroll
                     for (int ch = 0; ch < 8; ++ch)
@@ -1013,25 +1055,43 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
         }
 
         if constexpr (EPI == kXGatedBwd) {
-            // acc: the gradient of h. The three outputs' scales come from bounds,
-            // |dgate| <= 1.13 max|dh| max|up|, |dup| <= max|dh| max|gate|,
-            // |h| <= max|gate| max|up|: a scale a few powers of two above the tightest one moves
-            // the range of a floating format, not its precision, and saves a pass.
-            uint32_t* slot = red + parity * 4;
+            // acc: the gradient of h. The three outputs' scales come from bounds, the largest over
+            // a block's rows of
+            // |dgate| <= 1.13 max|dh| max|up|, |dup| <= max|dh| max|gate|, |h| <= max|gate| max|up|
+            // (the maxima over the row's 64 columns): a scale a few powers of two above the
+            // tightest one moves the range of a floating format, not its precision, and saves a
+            // pass. A row without a gradient has no part in any sum over rows, whatever is in it:
+            // its h is left out, and its size does not count.
+            uint32_t* slot = red + parity * 8;
+            const int grow = i * kXBlk + row;
+            const bool live = grow < g.m && g.live[grow] != 0;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                x_max_into(slot + b, largest<64>(acc + b * 64));
+                const int jb = w.tn * NB + b;
+                if (row_block && jb < g.nb) {
+                    const float* from = g.gmax +
+                                        static_cast<long long>(i * g.o[0].ldb + jb) * 4 * kXBlk +
+                                        half * kXBlk + row;
+                    const float gm = live ? from[0] : 0.0f, um = live ? from[2 * kXBlk] : 0.0f;
+                    const float dm = largest<64>(acc + b * 64);
+                    const float top = 3.402823466e38f;
+                    x_max_into(slot + b * 3, fminf(dm * um * kXMaxSlope, top));
+                    x_max_into(slot + b * 3 + 1, fminf(dm * gm, top));
+                    x_max_into(slot + b * 3 + 2, fminf(gm * um, top));
+                }
             }
             parity = parity == 2 ? 0 : parity + 1;
-            if (et < 4) red[parity * 4 + et] = 0u;
+            if (et < 8) red[parity * 8 + et] = 0u;
             epi_bar();
-            uint32_t top_of[3] = {slot[0], slot[1], slot[2]};
+            uint32_t top_of[NB * 3];
+#pragma unroll
+            for (int e = 0; e < NB * 3; ++e) top_of[e] = slot[e];
             if constexpr (SPL) {
                 cluster_sync();
                 for (int r = 0; r < g.splits; ++r) {
                     const uint32_t at = mapa_shared(slot, r * CG + rank);
 #pragma unroll
-                    for (int e = 0; e < 3; ++e)
+                    for (int e = 0; e < NB * 3; ++e)
                         top_of[e] = max(top_of[e], ld_cluster_u32(at + e * 4));
                 }
             }
@@ -1040,13 +1100,10 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
                 const int jb = w.tn * NB + b;
                 if (row_block && jb < g.nb) {
                     const int blk = i * g.o[0].ldb + jb;
-                    const float dm = __uint_as_float(top_of[b]);
-                    const float gm = g.gmax[blk * 2], um = g.gmax[blk * 2 + 1];
                     float s0, s1, s2, i0, i1, i2;
-                    const float top = 3.402823466e38f;
-                    split_scale(fminf(dm * um * kXMaxSlope, top), s0, i0);
-                    split_scale(fminf(dm * gm, top), s1, i1);
-                    split_scale(fminf(gm * um, top), s2, i2);
+                    split_scale(__uint_as_float(top_of[b * 3]), s0, i0);
+                    split_scale(__uint_as_float(top_of[b * 3 + 1]), s1, i1);
+                    split_scale(__uint_as_float(top_of[b * 3 + 2]), s2, i2);
                     if (et == 0 && w.s == 0) {
                         g.o[0].inv[blk] = i0;
                         g.o[1].inv[blk] = i1;
@@ -1072,7 +1129,7 @@ with_act(g.act, [&](auto kind) {
                             const float2 as = act_slope<decltype(kind)::value>(gs[x]);
                             dg[x] = dh * us[x] * as.y;
                             du[x] = dh * as.x;
-                            hh[x] = as.x * us[x];
+                            hh[x] = live ? as.x * us[x] : 0.0f;
                         }
                         store_split8(g.o[0].data + off, half * 8 + ch0 + ch, row, dg, s0);
                         store_split8(g.o[1].data + off, half * 8 + ch0 + ch, row, du, s1);
@@ -1103,7 +1160,7 @@ __global__ void __launch_bounds__(kXThreads, 1)
     uint64_t* tempty = tfull + 2;
     uint64_t* drain = tempty + 2;
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain + 1);
-    uint32_t* red = tmem_holder + 1;                       // three sets of four block maxima
+    uint32_t* red = tmem_holder + 1;                       // three sets of eight block maxima
     // the cluster barriers that the epilogue warps of an SPL kernel meet at
     constexpr int kSplitSyncs = !SPL ? 0 : EPI == kXF32 ? 2 : 3;
 
@@ -1124,7 +1181,7 @@ __global__ void __launch_bounds__(kXThreads, 1)
             mbar_init(&tempty[s], 8 * CG);
         }
         mbar_init(drain, 1);
-        for (int s = 0; s < 12; ++s) red[s] = 0u;
+        for (int s = 0; s < 24; ++s) red[s] = 0u;
         fence_barrier_init();
     }
     if (warp == 0 && lane == 0) {

@@ -45,3 +45,96 @@ def test_lookup_and_gradient(cuda, n, rows, d, dtype):
     close(got, grad, ids, rows, 1.7)
     assert torch.equal(got, mf.embedding_grad(grad, ids, rows, 1.7))   # the same bits again
     assert mf.device_status() == 0
+
+
+def test_shapes_views_and_padding(cuda):
+    g = torch.Generator(device="cuda").manual_seed(2)
+    table = torch.randn(50, 40, generator=g, device=cuda)
+    ids = torch.randint(0, 50, (3, 7, 5), generator=g, device=cuda)
+    grad = torch.randn(3, 7, 5, 40, generator=g, device=cuda)
+    for t in (table, torch.randn(50, 60, device=cuda)[:, 3:43].copy_(table),
+              table.t().contiguous().t()):
+        assert torch.equal(mf.embedding(t, ids), table[ids])
+    one = table[:1].expand(50, 40)
+    assert torch.equal(mf.embedding(one, ids), one[ids])
+    assert mf.embedding(table, ids.transpose(0, 2)).equal(table[ids.transpose(0, 2)])
+    assert mf.embedding(table, torch.tensor(7, device=cuda)).shape == (40,)
+    for view in (grad, torch.cat([grad, grad], -1)[..., :40],
+                 grad.permute(3, 0, 1, 2).contiguous().permute(1, 2, 3, 0)):
+        close(mf.embedding_grad(view, ids, 50, -0.5), grad, ids, 50, -0.5)
+    padded = mf.embedding_grad(grad, ids, 50, padding=3)
+    close(padded, grad, ids, 50, 1.0, padding=3)
+    assert (padded[3] == 0).all()
+    close(mf.embedding_grad(grad[0, 0, :1].expand(9, 40), ids.reshape(-1)[:9], 50),
+          grad[0, 0, :1].expand(9, 40), ids.reshape(-1)[:9], 50, 1.0)
+    assert mf.device_status() == 0
+
+
+def test_empty(cuda):
+    table = torch.randn(5, 4, device=cuda)
+    none = torch.empty(0, dtype=torch.int64, device=cuda)
+    assert mf.embedding(table, none).shape == (0, 4)
+    assert (mf.embedding_grad(torch.empty(0, 4, device=cuda), none, 5) == 0).all()
+    assert mf.embedding_grad(torch.empty(0, 4, device=cuda), none, 0).shape == (0, 4)
+    assert mf.embedding(torch.empty(5, 0, device=cuda), none.new_zeros(3)).shape == (3, 0)
+
+
+def test_ids_outside_the_table(cuda):
+    """Zeros for the lookup, no part in the gradient, a bit in the device's error word, and no
+    effect on kernels that wait (the bit is kept apart from theirs)."""
+    table = torch.randn(10, 36, device=cuda)
+    ids = torch.tensor([0, 10, -1, 9, 2 ** 40, 3], device=cuda)
+    good = torch.tensor([True, False, False, True, False, True], device=cuda)
+    grad = torch.randn(6, 36, device=cuda)
+    y = mf.embedding(table, ids)
+    assert torch.equal(y[good], table[ids[good]]) and (y[~good] == 0).all()
+    a = torch.randn(300, 64, device=cuda)
+    assert torch.isfinite(mf.gemm(a, a, transpose_b=True)).all()
+    assert mf.device_status() == 0x20
+    close(mf.embedding_grad(grad, ids, 10), grad, ids, 10, 1.0)
+    assert mf.device_status() == 0x20
+    assert mf.device_status() == 0
+    close(mf.embedding_grad(grad[:1], ids[:1], 10), grad[:1], ids[:1], 10, 1.0)
+    assert mf.device_status() == 0
+
+
+@pytest.mark.parametrize("n", [300, 70000])
+def test_one_id_and_every_id(cuda, n):
+    """All tokens of one id (the longest run there is), and each id once (runs of one)."""
+    grad = torch.randn(n, 12, device=cuda)
+    same = torch.full((n,), 4, device=cuda)
+    close(mf.embedding_grad(grad, same, 9), grad, same, 9, 1.0)
+    each = torch.randperm(n, device=cuda)
+    assert torch.equal(mf.embedding_grad(grad, each, n)[each], grad)
+
+
+def test_streams_and_graphs(cuda):
+    g = torch.Generator(device="cuda").manual_seed(6)
+    table = torch.randn(3000, 64, generator=g, device=cuda)
+    ids = torch.randint(0, 3000, (5000,), generator=g, device=cuda)
+    grad = torch.randn(5000, 64, generator=g, device=cuda)
+    both = lambda: (mf.embedding(table, ids, 2.0), mf.embedding_grad(grad, ids, 3000, 2.0))  # noqa: E731
+    plain = both()
+    side = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s in side:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got += [both() for _ in range(3)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for r in got for a, b in zip(r, plain))
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(both())
+        graphs.append(graph)
+    for _ in range(3):
+        ids.random_(0, 3000, generator=g)
+        grad.normal_(generator=g)
+        expect = both()
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for o in outs for a, b in zip(o, expect))
+    assert mf.device_status() == 0

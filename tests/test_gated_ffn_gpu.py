@@ -128,3 +128,211 @@ def test_weights_stored_outputs_first(cuda, rows, d, f):
         assert got.shape == w.shape and got.is_contiguous()
         close(got.t(), ref[name], name)
     assert mf.device_status() == 0
+
+
+@pytest.mark.parametrize("shape", [(600, 700, 900), (2100, 260, 1300), (640, 2048, 300)])
+def test_larger_tiles(cuda, shape):
+    """Sizes that fill 256 x 256 tiles, share contractions in clusters and leave ragged ends."""
+    x, wg, wu, wd, dy = inputs(cuda, *shape)
+    ref = want(x, wg, wu, wd, dy, "gelu")
+    y, saved = mf.gated_ffn(x, wg, wu, wd, "gelu", save=True)
+    close(y, ref["y"], "y")
+    grads = mf.gated_ffn_backward(dy, x, wg, wu, wd, "gelu", saved=saved)
+    for got, name in zip(grads, ("dx", "dwg", "dwu", "dwd")):
+        close(got, ref[name], name)
+    assert mf.device_status() == 0
+
+
+@pytest.mark.parametrize("rows", [1, 6, 16, 50, 300])
+def test_views(cuda, rows):
+    """Sliced, transposed and stepped tensors give what their packed copies give, bit for bit where
+    the same kernel runs, and gradients of leading dimensions fold."""
+    d, f = 132, 260
+    x, wg, wu, wd, dy = inputs(cuda, rows, d, f)
+    wide = torch.randn(rows, d + 9, device=cuda)
+    wide[:, 4:4 + d] = x
+    big = torch.randn(d, f + 13, device=cuda)
+    big[:, 5:5 + f] = wg
+    views = {
+        "sliced rows": (wide[:, 4:4 + d], wg, wu, wd),
+        "sliced weights": (x, big[:, 5:5 + f], wu, wd),
+        "column-major weights": (x, wg.t().contiguous().t(), wu.t().contiguous().t(),
+                                 wd.t().contiguous().t()),
+        "one of each": (x, wg.t().contiguous().t(), wu, wd),
+        "column-major rows": (x.t().contiguous().t(), wg, wu, wd),
+        "stepped": (torch.repeat_interleave(x, 2, 1)[:, ::2], wg, wu, wd),
+    }
+    ref = want(x, wg, wu, wd, dy, "silu")
+    few = want(x, wg, wu, wd, dy, "silu", few_rows) if rows <= 16 else ref
+    for name, (a, b, c, e) in views.items():
+        assert torch.equal(a, x) and torch.equal(b, wg)
+        close(mf.gated_ffn(a, b, c, e), few["y"], name)
+        y, saved = mf.gated_ffn(a, b, c, e, save=True)
+        close(y, ref["y"], name)
+        grads = mf.gated_ffn_backward(dy.t().contiguous().t(), a, b, c, e, saved=saved)
+        for got, key in zip(grads, ("dx", "dwg", "dwu", "dwd")):
+            assert got.is_contiguous()
+            close(got, ref[key], f"{name} {key}")
+    if rows % 2 == 0:
+        three = x.view(2, rows // 2, d)
+        y = mf.gated_ffn(three, wg, wu, wd)
+        assert y.shape == three.shape
+        close(y.reshape(rows, d), few["y"], "three dimensions")
+        dx = mf.gated_ffn_backward(dy.view_as(three), three, wg, wu, wd, need_w=False)[0]
+        assert dx.shape == three.shape
+        close(dx.reshape(rows, d), ref["dx"], "three dimensions dx")
+    vector = mf.gated_ffn(x[0], wg, wu, wd)
+    assert vector.shape == (d,)
+    assert mf.device_status() == 0
+
+
+def test_needed_gradients_only(cuda):
+    x, wg, wu, wd, dy = inputs(cuda, 140, 130, 200)
+    full = mf.gated_ffn_backward(dy, x, wg, wu, wd)
+    dx, *none = mf.gated_ffn_backward(dy, x, wg, wu, wd, need_w=False)
+    assert none == [None] * 3 and torch.equal(dx, full[0])
+    no_x, *dw = mf.gated_ffn_backward(dy, x, wg, wu, wd, need_x=False)
+    assert no_x is None and all(torch.equal(a, b) for a, b in zip(dw, full[1:]))
+    assert mf.gated_ffn_backward(dy, x, wg, wu, wd, need_x=False, need_w=False) == (None,) * 4
+
+
+def test_empty(cuda):
+    e = lambda *s: torch.empty(*s, device=cuda)  # noqa: E731
+    x, wg, wu, wd, _ = inputs(cuda, 3, 20, 30)
+    assert mf.gated_ffn(e(0, 20), wg, wu, wd).shape == (0, 20)
+    assert mf.gated_ffn(e(2, 0, 20), wg, wu, wd).shape == (2, 0, 20)
+    y, saved = mf.gated_ffn(e(0, 20), wg, wu, wd, save=True)
+    dx, *dw = mf.gated_ffn_backward(e(0, 20), e(0, 20), wg, wu, wd, saved=saved)
+    assert dx.shape == (0, 20) and all((t == 0).all() for t in dw)
+    assert all(t.shape == w.shape for t, w in zip(dw, (wg, wu, wd)))
+    zero = mf.gated_ffn(x, e(20, 0), e(20, 0), e(0, 20))          # no features: zeros
+    assert zero.shape == (3, 20) and (zero == 0).all()
+    dx, *dw = mf.gated_ffn_backward(x, x, e(20, 0), e(20, 0), e(0, 20))
+    assert (dx == 0).all() and [tuple(t.shape) for t in dw] == [(20, 0), (20, 0), (0, 20)]
+    assert mf.gated_ffn(e(4, 0), e(0, 30), e(0, 30), e(30, 0)).shape == (4, 0)
+    assert mf.device_status() == 0
+
+
+@pytest.mark.parametrize("rows", [9, 77, 700])
+def test_rows_do_not_depend_on_one_another(cuda, rows):
+    """A batch's rows keep their bits whatever the others hold: huge values, infinities, NaN."""
+    x, wg, wu, wd, dy = inputs(cuda, rows, 101, 203)
+    y = mf.gated_ffn(x, wg, wu, wd)
+    half = rows // 2
+    for filler in (1e6, 1e30, float("inf"), float("nan")):
+        other = x.clone()
+        other[half:] = filler
+        got = mf.gated_ffn(other, wg, wu, wd)
+        assert torch.equal(got[:half], y[:half]), filler
+        if filler > 1e30 or filler != filler:
+            assert not torch.isfinite(got[half:]).any()
+    one = x.clone()
+    one[3, 7] = float("inf")
+    got = mf.gated_ffn(one, wg, wu, wd)
+    assert not torch.isfinite(got[3]).any()
+    keep = [i for i in range(rows) if i != 3]
+    assert torch.equal(got[keep], y[keep])
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu", None])
+def test_rows_without_a_gradient_take_no_part(cuda, act):
+    """A padded batch: rows whose gradient is zero add nothing, whatever lies in them."""
+    x, wg, wu, wd, dy = inputs(cuda, 210, 130, 190)
+    dy[150:] = 0
+    ref = want(x[:150], wg, wu, wd, dy[:150], act)
+    for filler in (0.0, 3.0, 1e6, 1e30):
+        x[150:] = filler
+        for keep in (True, False):
+            saved = mf.gated_ffn(x, wg, wu, wd, act, save=True)[1] if keep else None
+            dx, *dw = mf.gated_ffn_backward(dy, x, wg, wu, wd, act, saved=saved)
+            assert (dx[150:] == 0).all()
+            close(dx[:150], ref["dx"], f"dx {filler}")
+            for got, name in zip(dw, ("dwg", "dwu", "dwd")):
+                close(got, ref[name], f"{name} {filler}")
+    assert mf.device_status() == 0
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-12, 1e12, 1e25])
+def test_scales(cuda, scale):
+    """Magnitudes far from 1: the scales carry them. The gate is x w_gate in both, the up projection
+    scales with x in the first call."""
+    x, wg, wu, wd, dy = inputs(cuda, 200, 96, 160)
+    y = mf.gated_ffn(x * scale, wg / scale, wu, wd, "relu")
+    ref = want(x, wg, wu, wd, dy, "relu")["y"]
+    close(y.double() / scale, (ref[0], ref[1] * 1.01), f"x {scale}")
+    y = mf.gated_ffn(x, wg, wu / scale, wd * scale, "relu")
+    close(y, (ref[0], ref[1] * 1.01), f"w_down {scale}")
+
+
+def test_gradients_against_differences(cuda):
+    """Central differences of the loss in 64 bits of the inputs' own values, along random
+    directions: the step's error is of order h^2, about 1e-5 of the derivative here."""
+    x, wg, wu, wd, dy = inputs(cuda, 150, 40, 70)
+    grads = mf.gated_ffn_backward(dy, x, wg, wu, wd, "gelu_tanh")
+
+    def loss(tensors):
+        a, b, c, e = tensors
+        act, _ = act64(a @ b, "gelu_tanh")
+        return float((((act * (a @ c)) @ e) * dy.double()).sum())
+
+    base = [t.double() for t in (x, wg, wu, wd)]
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    for i, g in enumerate(grads):
+        step = torch.randn(base[i].shape, generator=gen, device=cuda, dtype=torch.float64)
+        h = 1e-4
+        plus = [t + h * step if j == i else t for j, t in enumerate(base)]
+        minus = [t - h * step if j == i else t for j, t in enumerate(base)]
+        slope = (loss(plus) - loss(minus)) / (2 * h)
+        size = float((g.double().abs() * step.abs()).sum())
+        assert abs(float((g.double() * step).sum()) - slope) <= 1e-5 * size
+
+
+def test_streams_and_graphs(cuda):
+    """On another stream, two streams at once, and captured into two graphs that replay in turn
+    with new inputs: the results of plain calls, bit for bit."""
+    x, wg, wu, wd, dy = inputs(cuda, 200, 130, 300)
+    few = x[:4].contiguous()
+
+    def everything(a, b, g):
+        y, saved = mf.gated_ffn(a, wg, wu, wd, save=True)
+        return (y, mf.gated_ffn(b, wg, wu, wd)) + mf.gated_ffn_backward(g, a, wg, wu, wd,
+                                                                      saved=saved)
+
+    plain = everything(x, few, dy)
+    side = [torch.cuda.Stream() for _ in range(2)]
+    results = []
+    for s in side:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        for s in side:
+            with torch.cuda.stream(s):
+                results.append(everything(x, few, dy))
+    torch.cuda.synchronize()
+    for r in results:
+        assert all(torch.equal(a, b) for a, b in zip(r, plain))
+    ax, ag = x.clone(), dy.clone()
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(everything(ax, ax[:4], ag))
+        graphs.append(g)
+    for seed in range(3):
+        nx, _, _, _, ng = inputs(cuda, 200, 130, 300, seed + 1)
+        ax.copy_(nx)
+        ag.copy_(ng)
+        expect = everything(ax, ax[:4], ag)
+        for g, out in zip(graphs, outs):
+            g.replay()
+        torch.cuda.synchronize()
+        for out in outs:
+            assert all(torch.equal(a, b) for a, b in zip(out, expect))
+    assert mf.device_status() == 0
+
+
+def test_repeated_calls_give_the_same_bits(cuda):
+    x, wg, wu, wd, dy = inputs(cuda, 700, 900, 500)
+    first = mf.gated_ffn_backward(dy, x, wg, wu, wd)
+    for _ in range(3):
+        assert all(torch.equal(a, b)
+                   for a, b in zip(first, mf.gated_ffn_backward(dy, x, wg, wu, wd)))

@@ -60,3 +60,83 @@ def test_batches(cuda, shape):
     alone = torch.stack([mf.orthogonalize(m) for m in u])     # a batch is its matrices
     close(alone, want(u))
     assert mf.device_status() == 0
+
+
+def test_views_steps_and_coefficients(cuda):
+    g = torch.Generator(device="cuda").manual_seed(3)
+    u = torch.randn(3, 150, 70, generator=g, device=cuda)
+    big = torch.randn(3, 160, 90, generator=g, device=cuda)
+    big[:, 7:157, 5:75] = u
+    for view in (big[:, 7:157, 5:75], u.mT.contiguous().mT, u.transpose(0, 1).contiguous().transpose(0, 1),
+                 torch.repeat_interleave(u, 2, 2)[..., ::2]):
+        assert torch.equal(view, u)
+        close(mf.orthogonalize(view), want(u))
+    for steps in (1, 2, 7):
+        close(mf.orthogonalize(u, steps), want(u, steps))
+    c = (1.5, -0.5, 0.0)                                   # the cubic iteration
+    close(mf.orthogonalize(u, 12, c), want(u, 12, c))
+    close(mf.orthogonalize(u[0].expand(4, 150, 70)), want(u[0].expand(4, 150, 70)))
+    one = mf.orthogonalize(u[0].t())
+    close(one, want(u[0].t()))
+    large = torch.randn(520, 300, generator=g, device=cuda)
+    for view in (large.t(), large.t().contiguous().t()):
+        close(mf.orthogonalize(view), want(view))
+
+
+def test_scales_zero_and_nonfinite(cuda):
+    g = torch.Generator(device="cuda").manual_seed(4)
+    for shape in ((60, 100), (200, 400)):
+        u = torch.randn(*shape, generator=g, device=cuda)
+        ref = want(u)
+        for scale in (1e-3, 1e3, 1e25, 1e30):              # eps is negligible beside the norm
+            close(mf.orthogonalize(u * scale), ref)
+        close(mf.orthogonalize(u * 1e-25, eps=0.0), ref)
+        assert (mf.orthogonalize(torch.zeros_like(u)) == 0).all()
+        bad = torch.stack([u, u, u])
+        bad[1, 3, 5] = float("nan")
+        got = mf.orthogonalize(bad)
+        assert torch.isnan(got[1]).all()
+        close(got[::2], torch.stack([ref, ref]))
+    assert mf.device_status() == 0
+
+
+def test_empty(cuda):
+    assert mf.orthogonalize(torch.empty(0, 5, device=cuda)).shape == (0, 5)
+    assert mf.orthogonalize(torch.empty(0, 3, 5, device=cuda)).shape == (0, 3, 5)
+
+
+def test_singular_values_gather_around_one(cuda):
+    g = torch.Generator(device="cuda").manual_seed(9)
+    u = torch.randn(256, 1000, generator=g, device=cuda)
+    s = torch.linalg.svdvals(mf.orthogonalize(u).double())
+    assert 0.6 < float(s.min()) and float(s.max()) < 1.3
+
+
+@pytest.mark.parametrize("shape", [(2, 90, 120), (300, 700)])
+def test_streams_and_graphs(cuda, shape):
+    g = torch.Generator(device="cuda").manual_seed(1)
+    u = torch.randn(*shape, generator=g, device=cuda)
+    plain = mf.orthogonalize(u)
+    side = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s in side:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got += [mf.orthogonalize(u) for _ in range(3)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(r, plain) for r in got)
+    held = u.clone()
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(mf.orthogonalize(held))
+        graphs.append(graph)
+    for _ in range(3):
+        held.normal_(generator=g)
+        expect = mf.orthogonalize(held)
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, expect) for o in outs)
+    assert mf.device_status() == 0
