@@ -609,8 +609,7 @@ int run_orthogonalize(const float* u, int64_t batch, int64_t rows, int64_t cols,
     XMat x0;
     if (!x_source(ws, list, &x0, u, rows, cols, rs, 1, batch, bs)) return MFK_ERR_UNSUPPORTED;
     XMat x1 = steps > 1 ? x_mat(ws, rows, cols, batch) : x0;
-    const XMat gram = x_mat(ws, k, k, batch), quad = x_mat(ws, k, k, batch),
-               poly = x_mat(ws, k, k, batch);
+    const XMat gram = x_mat(ws, k, k, batch), poly = x_mat(ws, k, k, batch);
     rc = x_allocate(ws, 0);
     if (rc != MFK_OK) return rc;
     const XMat* mats[1] = {&x0};
@@ -634,35 +633,31 @@ int run_orthogonalize(const float* u, int64_t batch, int64_t rows, int64_t cols,
     }
     XMat *x = &x0, *next = &x1;
     for (int step = 0; step < steps; ++step) {
-        // With g the Gram matrix, a x + (b g + c g g) x = (a I + g (b I + c g)) x: the diagonals go
-        // into the factors as they are written, and no product reads a third matrix.
-        {   // gram = x x^T (or x^T x), quad = b I + c gram: symmetric, lower blocks only
+        {   // gram = x x^T (or x^T x): symmetric, lower blocks only
             mfk::XArgs g{};
             g.a[0] = g.a[1] = g.b[0] = g.b[1] = x_operand(ws, *x, !tall);
             g.mb = g.nb = gram.rb;
             g.m = g.n = static_cast<int>(k);
             g.sym = 1;
             g.o[0] = x_out(ws, gram);
-            g.o[1] = x_out(ws, quad);
-            g.second = 1;
-            g.scale1 = cc;
-            g.diag1 = cb;
             rc = x_product<mfk::kXSplit>(ws, g, depth, 0, batch);
             if (rc != MFK_OK) return rc;
         }
-        {   // poly = a I + gram quad: symmetric too
+        {   // poly = cb gram + cc gram gram
             mfk::XArgs g{};
-            g.a[0] = g.a[1] = x_operand(ws, gram, true, true);
-            g.b[0] = g.b[1] = x_operand(ws, quad, true, true);
+            g.a[0] = g.a[1] = g.b[0] = g.b[1] = x_operand(ws, gram, true, true);
             g.mb = g.nb = gram.rb;
             g.m = g.n = static_cast<int>(k);
             g.sym = 1;
+            g.alpha = cc;
+            g.beta = cb;
+            g.c = x_out(ws, gram);
             g.o[0] = x_out(ws, poly);
-            g.diag0 = ca;
             rc = x_product<mfk::kXSplit>(ws, g, k, 0, batch);
             if (rc != MFK_OK) return rc;
         }
-        // x = poly x (or x poly)
+        // x = ca x + poly x (or x poly). (With ca on poly's diagonal no third matrix is read, but then
+        // the largest term is rounded toward zero with the rest: 2.2e-6 off after five steps, not 8e-7.)
         mfk::XArgs g{};
         if (tall) {
             g.a[0] = g.a[1] = x_operand(ws, *x, true);
@@ -675,6 +670,9 @@ int run_orthogonalize(const float* u, int64_t batch, int64_t rows, int64_t cols,
         g.nb = x->cb;
         g.m = static_cast<int>(rows);
         g.n = static_cast<int>(cols);
+        g.alpha = 1.0f;
+        g.beta = ca;
+        g.c = x_out(ws, *x);
         if (step + 1 < steps) {
             g.o[0] = x_out(ws, *next);
             rc = x_product<mfk::kXSplit>(ws, g, k, 0, batch);

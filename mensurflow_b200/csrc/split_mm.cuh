@@ -71,9 +71,8 @@ struct XArgs {
     int m, n;              // output entries
     int tiles_m, tiles_n, splits, units, sym;
     int tiles;             // per matrix
-    // split output: o[0] = acc + diag0 I, and with `second` o[1] = scale1 acc + diag1 I
-    int second;
-    float diag0, scale1, diag1;
+    float alpha, beta;     // acc * alpha + C * beta
+    XOut c;                // C as a split matrix (beta != 0)
     float* out;            // fp32 output, row stride ld, batch stride out_bs
     long long ld, out_bs;
     XOut o[3];             // split outputs: result / h; dgate, dup, h
@@ -740,24 +739,40 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
         // this CTA's groups of eight columns: ng of them from ch0
         const int ch0 = SPL ? 8 * w.s / g.splits : 0;
         const int ng = SPL ? 8 * (w.s + 1) / g.splits - ch0 : 8;
-        // Backward: gate and up come eight columns (a turn) at a time through two slots of the
-        // warp's box, each lane copying what it reads itself, two turns ahead; the first two turns
-        // while the product is still computed, and the rest of the tile into L2 by then.
-        const int turns = EPI == kXGatedBwd && i < g.mb ? min(NB, g.nb - w.tn * NB) * ng : 0;
+        // What the epilogue reads comes eight columns (a turn) at a time through slots of the
+        // warp's box, each lane copying what it reads itself: the backward's gate and up in two
+        // slots, a split C in four. The first turns while the product is still computed (C read
+        // when it was needed made the tail of a 1024 x 4096 product 6 us instead of 4).
+        constexpr int kSlots = EPI == kXGatedBwd ? 2 : 4;
+        const bool reads = EPI == kXGatedBwd || (EPI != kXGated && g.beta != 0.0f);
+        const int turns = reads && i < g.mb ? min(NB, g.nb - w.tn * NB) * ng : 0;
         auto fetch = [&](int turn) {
             if (turn < turns) {
                 const int b = SPL ? turn / ng : turn >> 3, ch = turn - b * ng;
-                const long long at =
-                    ((static_cast<long long>(i * g.o[0].ldb + w.tn * NB + b) * 2 + half) * 64 +
-                     (ch0 + ch) * 8) * kXBlk + row * 4;
-                const uint32_t dst = smem_u32(box) + (turn & 1) * 2048 + lane * 16;
-                cp_async_16(dst, g.gate + at);
-                cp_async_16(dst + 512, g.gate + at + 4 * kXBlk);
-                cp_async_16(dst + 1024, g.up + at);
-                cp_async_16(dst + 1536, g.up + at + 4 * kXBlk);
+                const uint32_t dst = smem_u32(box) + (turn % kSlots) * (4096 / kSlots) + lane * 16;
+                if constexpr (EPI == kXGatedBwd) {
+                    const long long at =
+                        ((static_cast<long long>(i * g.o[0].ldb + w.tn * NB + b) * 2 + half) * 64 +
+                         (ch0 + ch) * 8) * kXBlk + row * 4;
+                    cp_async_16(dst, g.gate + at);
+                    cp_async_16(dst + 512, g.gate + at + 4 * kXBlk);
+                    cp_async_16(dst + 1024, g.up + at);
+                    cp_async_16(dst + 1536, g.up + at + 4 * kXBlk);
+                } else {
+                    const int blk = w.z * g.c.bstride + i * g.c.ldb + w.tn * NB + b;
+                    const uint8_t* p = g.c.data + static_cast<long long>(blk) * kXBlockBytes +
+                                       (half * 8 + ch0 + ch) * kXLineBytes + row * 16;
+                    cp_async_16(dst, p);
+                    cp_async_16(dst + 512, p + kXBlockBytes / 2);
+                }
             }
             cp_async_commit();
         };
+        if (reads) {
+            __syncwarp();  // the box held the last tile's result
+#pragma unroll
+            for (int t = 0; t < kSlots; ++t) fetch(t);
+        }
         if constexpr (EPI == kXGatedBwd) {
             for (int b = 0; b < NB; ++b) {
                 const int jb = w.tn * NB + b;
@@ -769,8 +784,6 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
                     }
                 }
             }
-            fetch(0);
-            fetch(1);
         }
         float acc[NB * 64];
 #pragma unroll
@@ -860,6 +873,41 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
         }
         const bool row_block = i < g.mb;
 
+        if constexpr (EPI == kXF32 || EPI == kXSplit) {
+            if (reads) {  // alpha acc + beta C
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    const int jb = w.tn * NB + b;
+                    if (row_block && jb < g.nb) {
+                        const float f = g.c.inv[w.z * g.c.bstride + i * g.c.ldb + jb] * g.beta;
+#pragma unroll
+                        for (int ch = 0; ch < 8; ++ch) {
+                            if (SPL && ch >= ng) break;
+                            const int turn = b * ng + ch;
+                            const uint32_t src =
+                                smem_u32(box) + (turn % kSlots) * (4096 / kSlots) + lane * 16;
+                            cp_async_wait<kSlots - 1>();
+                            const float4 hq = ld_shared_v4(src), lq = ld_shared_v4(src + 512);
+                            fetch(turn + kSlots);
+                            const float hs[4] = {hq.x, hq.y, hq.z, hq.w};
+                            const float ls[4] = {lq.x, lq.y, lq.z, lq.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float2 hf =
+                                    __half22float2(*reinterpret_cast<const __half2*>(&hs[e]));
+                                const float2 lf =
+                                    __half22float2(*reinterpret_cast<const __half2*>(&ls[e]));
+                                float* v = acc + b * 64 + ch * 8 + e * 2;
+                                v[0] = fmaf(hf.x + lf.x, f, v[0] * g.alpha);
+                                v[1] = fmaf(hf.y + lf.y, f, v[1] * g.alpha);
+                            }
+                        }
+                    }
+                }
+                cp_async_wait<0>();
+            }
+        }
+
         if constexpr (EPI == kXF32 && SPL) {
             const int grow = i * kXBlk + row;
 #pragma unroll
@@ -931,15 +979,8 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
 
         if constexpr (EPI == kXSplit) {
             uint32_t* slot = red + parity * 8;
-            // this thread's column, of those at the front of acc, on a diagonal block's diagonal
-            const int diag_at = row - half * 64 - ch0 * 8;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                if (g.diag0 != 0.0f && i == w.tn * NB + b) {
-#pragma unroll
-                    for (int j = 0; j < 64; ++j)
-                        if (j == diag_at && j < ng * 8) acc[b * 64 + j] += g.diag0;
-                }
                 x_max_into(slot + b, largest<64>(acc + b * 64));
             }
             parity = parity == 2 ? 0 : parity + 1;
@@ -960,34 +1001,14 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
                 const int jb = w.tn * NB + b;
                 if (row_block && jb < g.nb) {
                     float s, inv;
-                    const float top = __uint_as_float(top_of[b]);
                     const int blk = w.z * g.o[0].bstride + i * g.o[0].ldb + jb;
-                    split_scale(top, s, inv);
+                    split_scale(__uint_as_float(top_of[b]), s, inv);
                     if (et == 0 && w.s == 0) g.o[0].inv[blk] = inv;
                     uint8_t* dst = g.o[0].data + static_cast<long long>(blk) * kXBlockBytes;
 #pragma unroll
                     for (int ch = 0; ch < 8; ++ch)
                         if (ch < ng)
                             store_split8(dst, half * 8 + ch0 + ch, row, acc + b * 64 + ch * 8, s);
-                    if (g.second) {
-                        // its scale from a bound: no second maximum
-                        const int blk1 = w.z * g.o[1].bstride + i * g.o[1].ldb + jb;
-                        split_scale(fminf(fmaf(fabsf(g.scale1), top, fabsf(g.diag1)),
-                                          3.402823466e38f), s, inv);
-                        if (et == 0 && w.s == 0) g.o[1].inv[blk1] = inv;
-                        uint8_t* dst1 = g.o[1].data + static_cast<long long>(blk1) * kXBlockBytes;
-#pragma unroll
-                        for (int ch = 0; ch < 8; ++ch) {
-                            if (ch < ng) {
-                                float v[8];
-#pragma unroll
-                                for (int e = 0; e < 8; ++e)
-                                    v[e] = fmaf(acc[b * 64 + ch * 8 + e], g.scale1,
-                                                i == jb && ch * 8 + e == diag_at ? g.diag1 : 0.0f);
-                                store_split8(dst1, half * 8 + ch0 + ch, row, v, s);
-                            }
-                        }
-                    }
                 }
             }
         }
@@ -1116,11 +1137,12 @@ with_act(g.act, [&](auto kind) {
                         if (SPL && ch >= ng) break;
                         float dg[8], du[8], hh[8];
                         const int turn = b * ng + ch;
-                        const uint32_t src = smem_u32(box) + (turn & 1) * 2048 + lane * 16;
-                        cp_async_wait<1>();
+                        const uint32_t src =
+                            smem_u32(box) + (turn % kSlots) * (4096 / kSlots) + lane * 16;
+                        cp_async_wait<kSlots - 1>();
                         const float4 g0 = ld_shared_v4(src), g1 = ld_shared_v4(src + 512);
                         const float4 u0 = ld_shared_v4(src + 1024), u1 = ld_shared_v4(src + 1536);
-                        fetch(turn + 2);
+                        fetch(turn + kSlots);
                         const float gs[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
                         const float us[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
 #pragma unroll
