@@ -272,9 +272,18 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0) -> tor
     names, [*ids.shape, d]. An id outside the table gives a row of zeros and sets the bit
     ``MFK_DEVERR_INDEX`` of ``device_status()``."""
     op = "embedding"
-    _require(table, op, "table", 2)
-    index = _ids(op, ids, table)
-    _kernel_for(op, table)
+    try:  # the usual call, checked in one go
+        plain = (table.dtype is torch.float32 and table.is_cuda and table.dim() == 2 and
+                 ids.dtype in (torch.int64, torch.int32) and ids.device == table.device and
+                 ids.is_contiguous())
+    except AttributeError:
+        plain = False
+    if plain:
+        index = ids
+    else:
+        _require(table, op, "table", 2)
+        index = _ids(op, ids, table)
+        _kernel_for(op, table)
     rows, d = table.shape
     n = index.numel()
     if rows == 0 and n and d:

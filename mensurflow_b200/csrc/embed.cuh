@@ -168,6 +168,7 @@ __global__ void __launch_bounds__(256)
                         long long n, int shift, const uint32_t* __restrict__ offsets, int tiles,
                         uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out) {
     __shared__ uint32_t counts[8][257];
+    grid_dependents_go();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int i = threadIdx.x; i < 8 * 257; i += 256) (&counts[0][0])[i] = 0u;
     __syncthreads();
@@ -237,6 +238,7 @@ __global__ void __launch_bounds__(1024, 1)
     const int first = rank * chunk;
     const int count = max(0, min(chunk, n - first));
 
+    grid_dependents_go();
     const long long words = (rows + 31) / 32;
     for (long long i = rank * 1024 + static_cast<int>(threadIdx.x); i < words; i += ranks * 1024)
         present[i] = 0u;
@@ -386,11 +388,13 @@ constexpr int kEmbedMaxWindow = 256;
 // part[2 w + 1]. The blocks behind them write zeros into the rows that no token names, a warp per
 // row: they fill the memory system while the sums wait for their rows.
 __global__ void __launch_bounds__(256)
-    embed_sum_kernel(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
+    embed_sum_kernel(const uint32_t* keys, const uint32_t* pos,
                      long long n, int window, uint32_t rows, const float* __restrict__ grad,
                      long long ld_grad, int d, float scale, float* __restrict__ out, long long ld,
-                     float* __restrict__ part, int vec, int pieces, int sum_blocks,
-                     const uint32_t* __restrict__ present) {
+                     float* part, int vec, int pieces, int sum_blocks,
+                     const uint32_t* present) {
+    grid_dependents_go();
+    grid_wait();
     if (static_cast<int>(blockIdx.x) >= sum_blocks) {
         const int lane = threadIdx.x & 31;
         const int warps = (static_cast<int>(gridDim.x) - sum_blocks) * 8;
@@ -462,9 +466,10 @@ __global__ void __launch_bounds__(256)
 
 // One block per window whose last run starts in it and goes on: the run's parts in order.
 __global__ void __launch_bounds__(256)
-    embed_join_kernel(const uint32_t* __restrict__ keys, long long n, int window, uint32_t rows,
+    embed_join_kernel(const uint32_t* keys, long long n, int window, uint32_t rows,
                       int d, float scale, float* __restrict__ out, long long ld,
-                      const float* __restrict__ part, int vec) {
+                      const float* part, int vec) {
+    grid_wait();
     const long long w = blockIdx.x;
     const long long next = (w + 1) * window;   // first token of the next window
     if (next >= n) return;

@@ -155,16 +155,29 @@ int run_embedding_grad(const float* grad, int64_t n, int64_t d, int64_t ld_grad,
     }
     const int sum_blocks = static_cast<int>(windows * pieces);
     const int64_t zero_blocks = std::min<int64_t>((rows + 7) / 8, int64_t(info->sm_count) * 64);
-    mfk::embed_sum_kernel<<<static_cast<unsigned>(sum_blocks + zero_blocks), 256, 0, stream>>>(
-        keys[at], pos[at], n, window, static_cast<uint32_t>(rows), grad, ld_grad,
-        static_cast<int>(d), scale, out, ld, d_part, vec, pieces, sum_blocks, d_marks);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cfg.blockDim = dim3(256, 1, 1);
+    cfg.stream = stream;
+    cfg.gridDim = dim3(static_cast<unsigned>(sum_blocks + zero_blocks), 1, 1);
+    const uint32_t *sorted = keys[at], *order = pos[at], *present = d_marks;
+    MFK_CUDA(cudaLaunchKernelEx(&cfg, mfk::embed_sum_kernel, sorted, order,
+                                static_cast<long long>(n), window, static_cast<uint32_t>(rows),
+                                grad, static_cast<long long>(ld_grad), static_cast<int>(d), scale,
+                                out, static_cast<long long>(ld), d_part, vec, pieces, sum_blocks,
+                                present));
     g_launches.fetch_add(1);
     if (windows > 1) {
-        const dim3 grid(static_cast<unsigned>(windows), static_cast<unsigned>(pieces), 1);
-        mfk::embed_join_kernel<<<grid, 256, 0, stream>>>(keys[at], n, window,
-                                                         static_cast<uint32_t>(rows),
-                                                         static_cast<int>(d), scale, out, ld,
-                                                         d_part, vec);
+        cfg.gridDim = dim3(static_cast<unsigned>(windows), static_cast<unsigned>(pieces), 1);
+        MFK_CUDA(cudaLaunchKernelEx(&cfg, mfk::embed_join_kernel, sorted,
+                                    static_cast<long long>(n), window,
+                                    static_cast<uint32_t>(rows), static_cast<int>(d), scale, out,
+                                    static_cast<long long>(ld), static_cast<const float*>(d_part),
+                                    vec));
         g_launches.fetch_add(1);
     }
     MFK_CUDA(cudaGetLastError());

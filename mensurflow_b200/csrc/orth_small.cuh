@@ -9,18 +9,22 @@
 //         rank order (every CTA adds all of them, so all hold the same g);
 //     p = b g + c g g;
 //     x = a x + p x.
-// Sums between products stay in fp32 registers (a thread has one row and 64 columns); only the
-// operands are split. Bound by latency: a product is 24 MMAs of 64 cycles and about as long again
-// for the way TMEM -> registers -> shared memory; 48 matrices of 64 x 128, five steps: 115 us as
-// seventeen launches of the general kernels.
+// Sums between products stay in fp32 registers (a thread has one row and 32 columns); only the
+// operands are split. Products are as wide and as deep as the matrix in steps of 16, and a thread
+// whose columns lie outside does nothing. Bound by latency: a product is up to 24 MMAs of 64 cycles
+// and longer again for the way TMEM -> registers -> shared memory; 48 matrices of 64 x 128, five
+// steps: 115 us as seventeen launches of the general kernels.
 #pragma once
 
 #include "split_mm.cuh"
 
 namespace mfk {
 
-constexpr int kOrthThreads = 288;          // eight warps with the rows, one that issues the MMAs
-constexpr int kOrthSmem = 3 * kXBlockBytes + 1024 + 256;
+constexpr int kOrthWarps = 16;             // with the values, and one that issues the MMAs
+constexpr int kOrthValues = kOrthWarps * 32;
+constexpr int kOrthThreads = kOrthValues + 32;
+constexpr int kOrthCols = 32;              // of a thread
+constexpr int kOrthSmem = 3 * kXBlockBytes + 1024 + 512;
 constexpr int kOrthMaxRanks = 8;
 
 struct OrthSmallArgs {
@@ -40,16 +44,16 @@ __device__ __forceinline__ double ld_cluster_f64(uint32_t addr) {
     return v;
 }
 
-// D (+)= A B over a depth of 128 (or 64 where the rest is zero): the lo products first.
+// D (128 x n) = A B over `depth`, both in steps of 16: the lo products first.
 __device__ __forceinline__ void orth_mma(uint32_t d, uint32_t a, int a_flip, uint32_t b, int b_flip,
-                                         int depth) {
+                                         int n, int depth) {
     // blocks with all 16 lines: K-major 2 KB apart along k, 128 B along rows; MN-major 128 B
     // along k, 2 KB along the other
     const uint32_t a_lbo = a_flip ? 128u : 2048u, a_sbo = a_flip ? 2048u : 128u;
     const uint32_t b_lbo = b_flip ? 128u : 2048u, b_sbo = b_flip ? 2048u : 128u;
     const uint32_t a_step = a_flip ? 256u : 4096u, b_step = b_flip ? 256u : 4096u;
-    const uint32_t idesc = idesc_f16(128, 128, a_flip != 0, b_flip != 0);
-    const int ks_end = depth <= 64 ? 4 : 8;
+    const uint32_t idesc = idesc_f16(128, (n + 15) / 16 * 16, a_flip != 0, b_flip != 0);
+    const int ks_end = (depth + 15) / 16;
     for (int ks = 0; ks < ks_end; ++ks) {
         const uint32_t sa = a + ks * a_step, sb = b + ks * b_step;
         const uint64_t ah = smem_desc(sa, a_lbo, a_sbo, kSwizzleNone);
@@ -64,29 +68,30 @@ __device__ __forceinline__ void orth_mma(uint32_t d, uint32_t a, int a_flip, uin
                    smem_desc(b + ks * b_step, b_lbo, b_sbo, kSwizzleNone), idesc, 1u);
 }
 
-__device__ __forceinline__ void orth_bar() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void orth_bar() { asm volatile("bar.sync 1, %0;" ::"n"(kOrthValues) : "memory"); }
 
-// The largest magnitude over the eight warps' values. Two sets of slots take turns; a set is next
+// The largest magnitude over all values. Two sets of slots take turns; a set is next
 // written two calls later, behind the barriers in between.
 __device__ __forceinline__ float orth_max(uint32_t* red, int& turn, float amax) {
-    uint32_t* slot = red + turn * 8;
+    uint32_t* slot = red + turn * kOrthWarps;
     turn ^= 1;
     const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(amax));
     if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = m;
     orth_bar();
-    uint32_t all = 0;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) all = max(all, slot[w]);
-    return __uint_as_float(all);
+    return __uint_as_float(
+        __reduce_max_sync(0xffffffffu, slot[threadIdx.x & (kOrthWarps - 1)]));
 }
 
-// v (one row, 64 columns a thread) as a split block in shared memory; returns 1/s.
-__device__ __forceinline__ float orth_split(uint8_t* block, const float* v, int half, int row,
-                                            uint32_t* red, int& turn) {
-    float s, inv;
-    split_scale(orth_max(red, turn, largest<64>(v)), s, inv);
+// v (one row, 32 columns a thread, the first `groups` x 16 of them in use) as a split block in
+// shared memory; returns 1/s.
+__device__ __forceinline__ float orth_split(uint8_t* block, const float* v, int part, int row,
+                                            int groups, uint32_t* red, int& turn) {
+    float s, inv, m = 0.0f;
+    if (groups > 0) m = largest<kOrthCols>(v);
+    split_scale(orth_max(red, turn, m), s, inv);
 #pragma unroll
-    for (int ch = 0; ch < 8; ++ch) store_split8(block, half * 8 + ch, row, v + ch * 8, s);
+    for (int ch = 0; ch < kOrthCols / 8; ++ch)
+        if (ch < groups * 2) store_split8(block, part * (kOrthCols / 8) + ch, row, v + ch * 8, s);
     fence_proxy_async_smem();
     return inv;
 }
@@ -101,8 +106,8 @@ __global__ void __launch_bounds__(kOrthThreads, 1)
     uint8_t* sp = base + 2 * kXBlockBytes;       // p, and before it the parts of g in fp32
     uint64_t* done = reinterpret_cast<uint64_t*>(base + 3 * kXBlockBytes);
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(done + 1);
-    uint32_t* red = tmem_holder + 2;             // two sets of eight
-    double* sums = reinterpret_cast<double*>(red + 16);  // eight warps, then this CTA's sum
+    uint32_t* red = tmem_holder + 2;             // two sets of slots
+    double* sums = reinterpret_cast<double*>(red + 2 * kOrthWarps);  // the warps', then the CTA's
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int ranks = static_cast<int>(cluster_nctarank());
     const int rank = static_cast<int>(cluster_ctarank());
@@ -113,14 +118,14 @@ __global__ void __launch_bounds__(kOrthThreads, 1)
         mbar_init(done, 1);
         fence_barrier_init();
     }
-    if (warp == 8) tmem_alloc(tmem_holder, 128);
+    if (warp == kOrthWarps) tmem_alloc(tmem_holder, 128);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_holder;
 
-    if (warp == 8) {
-        // One lane issues; the three barriers a step are the eight warps' word that the operands
+    if (warp == kOrthWarps) {
+        // One lane issues; the three barriers a step are the other warps' word that the operands
         // of the next product lie in shared memory.
         const uint32_t ax = smem_u32(sx), ag = smem_u32(sg), ap = smem_u32(sp);
         const int own = min(128, (g.tall ? g.rows : g.cols) - rank * 128);
@@ -132,13 +137,13 @@ __global__ void __launch_bounds__(kOrthThreads, 1)
                 if (lane == 0) {
                     tc_fence_after();
                     if (i == 0) {
-                        orth_mma(tmem, ax, g.tall, ax, g.tall, own);
+                        orth_mma(tmem, ax, g.tall, ax, g.tall, k, own);
                     } else if (i == 1) {
-                        orth_mma(tmem, ag, 0, ag, 0, k);
+                        orth_mma(tmem, ag, 0, ag, 0, k, k);
                     } else if (g.tall) {
-                        orth_mma(tmem, ax, 0, ap, 0, k);
+                        orth_mma(tmem, ax, 0, ap, 0, k, k);
                     } else {
-                        orth_mma(tmem, ap, 0, ax, 1, k);
+                        orth_mma(tmem, ap, 0, ax, 1, own, k);
                     }
                     mma_commit(done);
                 }
@@ -150,19 +155,23 @@ __global__ void __launch_bounds__(kOrthThreads, 1)
             }
         }
     } else {
-        const int q = warp % 4, half = warp / 4;
+        const int q = warp % 4, part = warp / 4;   // TMEM lanes, columns 32 part ..
         const int row = q * 32 + lane;
-        const uint32_t lanes = tmem + (static_cast<uint32_t>(q * 32) << 16) + half * 64;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(q * 32) << 16) + part * kOrthCols;
         const int r0 = g.tall ? rank * 128 : 0, c0 = g.tall ? 0 : rank * 128;
+        // this thread's sixteens of columns in use: of the k x k matrices, and of x
+        const int gk = max(0, min(2, (k - part * kOrthCols + 15) / 16));
+        const int own = g.tall ? k : min(128, g.cols - rank * 128);
+        const int gx = max(0, min(2, (own - part * kOrthCols + 15) / 16));
         int turn = 0;
         uint32_t phase = 0;
-        float x[64], acc[64];
+        float x[kOrthCols], acc[kOrthCols];
         // the block through shared memory, so that global rows are read along
         float* stage = reinterpret_cast<float*>(sg);     // [128][129], in g and p
         {
             const float* u = g.u + z * g.bs;
 #pragma unroll 8
-            for (int i = threadIdx.x; i < 128 * 128; i += 256) {
+            for (int i = threadIdx.x; i < 128 * 128; i += kOrthValues) {
                 const int r = i >> 7, c = i & 127;
                 const bool in = r0 + r < g.rows && c0 + c < g.cols;
                 stage[r * 129 + c] =
@@ -171,8 +180,8 @@ __global__ void __launch_bounds__(kOrthThreads, 1)
             orth_bar();
             double sum = 0.0;
 #pragma unroll
-            for (int j = 0; j < 64; ++j) {
-                x[j] = stage[row * 129 + half * 64 + j];
+            for (int j = 0; j < kOrthCols; ++j) {
+                x[j] = stage[row * 129 + part * kOrthCols + j];
                 sum += static_cast<double>(x[j]) * static_cast<double>(x[j]);
             }
 #pragma unroll
@@ -181,15 +190,15 @@ __global__ void __launch_bounds__(kOrthThreads, 1)
             orth_bar();
             if (threadIdx.x == 0) {
                 double t = 0.0;
-                for (int w = 0; w < 8; ++w) t += sums[w];
-                sums[8] = t;
+                for (int w = 0; w < kOrthWarps; ++w) t += sums[w];
+                sums[kOrthWarps] = t;
             }
             cluster_sync();
             double total = 0.0;
-            for (int r = 0; r < ranks; ++r) total += ld_cluster_f64(mapa_shared(sums + 8, r));
+            for (int r = 0; r < ranks; ++r) total += ld_cluster_f64(mapa_shared(sums + kOrthWarps, r));
             const float f = static_cast<float>(1.0 / (sqrt(total) + static_cast<double>(g.eps)));
 #pragma unroll
-            for (int j = 0; j < 64; ++j) x[j] *= f;
+            for (int j = 0; j < kOrthCols; ++j) x[j] *= f;
         }
         bool alive = true;  // a wait that gave up: finish without waiting, every barrier is met
         auto product_done = [&]() {
@@ -199,60 +208,66 @@ __global__ void __launch_bounds__(kOrthThreads, 1)
             tc_fence_after();
         };
         for (int step = 0; step < g.steps; ++step) {
-            const float xi = orth_split(sx, x, half, row, red, turn);
+            const float xi = orth_split(sx, x, part, row, gx, red, turn);
+            tc_fence_before();
             __syncthreads();
             product_done();
             // g
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
+            for (int t = 0; t < kOrthCols / 16; ++t) {
                 float r[16];
-                tmem_ld_32x32b_x16(lanes + t * 16, r);
+                if (t < gk) tmem_ld_32x32b_x16(lanes + t * 16, r);
 #pragma unroll
-                for (int j = 0; j < 16; ++j) acc[t * 16 + j] = (r[j] * xi) * xi;
+                for (int j = 0; j < 16; ++j) acc[t * 16 + j] = t < gk ? (r[j] * xi) * xi : 0.0f;
             }
             if (ranks > 1) {
-                float4* part = reinterpret_cast<float4*>(sp) + threadIdx.x;
+                float4* mine = reinterpret_cast<float4*>(sp) + threadIdx.x;
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    part[j * 256] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2],
-                                                acc[4 * j + 3]);
+                for (int j = 0; j < kOrthCols / 4; ++j)
+                    if (j < gk * 4)
+                        mine[j * kOrthValues] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2],
+                                                    acc[4 * j + 3]);
                 cluster_sync();
 #pragma unroll
-                for (int j = 0; j < 64; ++j) acc[j] = 0.0f;
+                for (int j = 0; j < kOrthCols; ++j) acc[j] = 0.0f;
                 for (int r = 0; r < ranks; ++r) {
-                    const uint32_t at = mapa_shared(part, r);
+                    const uint32_t at = mapa_shared(mine, r);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const float4 v = ld_cluster_v4(at + j * 4096);
-                        acc[4 * j] += v.x;
-                        acc[4 * j + 1] += v.y;
-                        acc[4 * j + 2] += v.z;
-                        acc[4 * j + 3] += v.w;
+                    for (int j = 0; j < kOrthCols / 4; ++j) {
+                        if (j < gk * 4) {
+                            const float4 v = ld_cluster_v4(at + j * kOrthValues * 16);
+                            acc[4 * j] += v.x;
+                            acc[4 * j + 1] += v.y;
+                            acc[4 * j + 2] += v.z;
+                            acc[4 * j + 3] += v.w;
+                        }
                     }
                 }
                 cluster_sync();
             }
-            const float gi = orth_split(sg, acc, half, row, red, turn);
+            const float gi = orth_split(sg, acc, part, row, gk, red, turn);
             tc_fence_before();
             __syncthreads();
             product_done();
             // p = b g + c g g
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
+            for (int t = 0; t < kOrthCols / 16; ++t) {
                 float r[16];
+                if (t >= gk) break;
                 tmem_ld_32x32b_x16(lanes + t * 16, r);
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
                     acc[t * 16 + j] = fmaf(g.b, acc[t * 16 + j], ((r[j] * gi) * gi) * g.c);
             }
-            const float pi = orth_split(sp, acc, half, row, red, turn);
+            const float pi = orth_split(sp, acc, part, row, gk, red, turn);
             tc_fence_before();
             __syncthreads();
             product_done();
             // x = a x + p x
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
+            for (int t = 0; t < kOrthCols / 16; ++t) {
                 float r[16];
+                if (t >= gx) break;
                 tmem_ld_32x32b_x16(lanes + t * 16, r);
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
@@ -262,11 +277,11 @@ __global__ void __launch_bounds__(kOrthThreads, 1)
         }
         // out, along the rows again
 #pragma unroll
-        for (int j = 0; j < 64; ++j) stage[row * 129 + half * 64 + j] = x[j];
+        for (int j = 0; j < kOrthCols; ++j) stage[row * 129 + part * kOrthCols + j] = x[j];
         orth_bar();
         float* out = g.out + z * g.out_bs;
 #pragma unroll 8
-        for (int i = threadIdx.x; i < 128 * 128; i += 256) {
+        for (int i = threadIdx.x; i < 128 * 128; i += kOrthValues) {
             const int r = i >> 7, c = i & 127;
             if (r0 + r < g.rows && c0 + c < g.cols)
                 out[static_cast<long long>(r0 + r) * g.ld + c0 + c] = stage[r * 129 + c];
@@ -274,7 +289,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1)
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == kOrthWarps) {
         tc_fence_after();
         tmem_dealloc(tmem, 128);
     }
