@@ -64,10 +64,11 @@ class GatedSaved:
     """What ``gated_ffn(..., save=True)`` keeps for the backward pass: the gate's and the up
     projection's results, in the kernels' own order, in a device tensor (``buffer``)."""
 
-    def __init__(self, buffer: torch.Tensor, rows: int, features: int):
+    def __init__(self, buffer: torch.Tensor, rows: int, features: int, activation):
         self.buffer = buffer
         self.rows = rows
         self.features = features
+        self.activation = activation
 
 
 def _gated_fast(x, w_gate, w_up, w_down, activation, transpose_w):
@@ -169,7 +170,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
     saved = None
     if save:
-        saved = GatedSaved(x.new_empty(so.mfk_gated_ffn_saved_floats(rows, f)), rows, f)
+        saved = GatedSaved(x.new_empty(so.mfk_gated_ffn_saved_floats(rows, f)), rows, f, activation)
     _run(x.device, "gated_ffn", so.mfk_gated_ffn_f32, ctypes.byref(desc), _ptr(y), d or 1,
          _ptr(saved.buffer) if save else None)
     return (y, saved) if save else y
@@ -195,9 +196,11 @@ def gated_ffn_backward(grad: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor
     if saved is not None:
         if not isinstance(saved, GatedSaved):
             raise TypeError(f"{op}: saved must come from gated_ffn(..., save=True)")
-        if (saved.rows, saved.features) != (rows, f) or saved.buffer.device != x.device:
+        if (saved.rows, saved.features) != (rows, f) or saved.buffer.device != x.device or \
+                saved.buffer.numel() != _lib.lib().mfk_gated_ffn_saved_floats(rows, f) or \
+                _GATED_ACTS[saved.activation] != desc.activation:
             raise ValueError(f"{op}: saved belongs to another call ({saved.rows} rows, "
-                             f"{saved.features} features)")
+                             f"{saved.features} features, {saved.activation})")
     if not need_x and not need_w:
         return None, None, None, None
     g2 = _rows_of(grad, rows, d)

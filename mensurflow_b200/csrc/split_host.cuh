@@ -264,9 +264,13 @@ int x_product(XWorkspace& ws, mfk::XArgs& g, int64_t k0, int64_t k1, int64_t bat
     const int64_t tiles2 = g.sym ? tm2 * (tm2 + 1) / 2 : tm2 * tn2;
     const int64_t tiles1 = g.sym ? tm1 * (tm1 + 1) / 2 : tm1 * tn1;
     if (tiles1 * batch > (int64_t(1) << 26)) return MFK_ERR_UNSUPPORTED;
-    // The backward epilogue has three outputs and two inputs, the gated one an activation.
-    constexpr double kEpi = EPI == mfk::kXGatedBwd ? 12000.0 : EPI == mfk::kXGated ? 6000.0
-                                                                                   : 3000.0;
+    // What the epilogue adds to a wave, measured at 8 chunks. The backward one has three outputs and
+    // two inputs, and no registers to spare beside a pair's 128 sums a thread: 4096 x 1024 x 4096
+    // takes 163 us by pairs and 154 by single CTAs (at 32 chunks the pairs win).
+    constexpr double kEpi1 = EPI == mfk::kXGatedBwd ? 10000.0 : EPI == mfk::kXGated ? 7000.0
+                                                                                    : 3000.0;
+    constexpr double kEpi2 = EPI == mfk::kXGatedBwd ? 30000.0 : EPI == mfk::kXGated ? 7000.0
+                                                                                    : 6000.0;
     // 256 x 256 by pairs of CTAs where there are tiles enough, 128-row tiles of one CTA where there
     // are not, and either with the contraction shared by a cluster where that leaves SMs idle.
     int slots = 0, best_slots = 0, pairs = 0, splits = 0, rc = MFK_OK;
@@ -286,13 +290,13 @@ int x_product(XWorkspace& ws, mfk::XArgs& g, int64_t k0, int64_t k1, int64_t bat
         rc = s == 1 ? x_slots<2, 2, EPI, false>(ws, EPI * 12 + s - 1, 2, &slots)
                     : x_slots<2, 2, EPI, true>(ws, EPI * 12 + s - 1, 2 * s, &slots);
         if (rc != MFK_OK) return rc;
-        consider(2, s, tiles2, 3072.0, kEpi * 2, 17000.0);
+        consider(2, s, tiles2, 3072.0, kEpi2, 17000.0);
     }
     for (int s = 1; s <= 8 && s <= g.kc; ++s) {
         rc = s == 1 ? x_slots<1, kNb1, EPI, false>(ws, EPI * 12 + 3 + s, 1, &slots)
                     : x_slots<1, kNb1, EPI, true>(ws, EPI * 12 + 3 + s, s, &slots);
         if (rc != MFK_OK) return rc;
-        consider(1, s, tiles1, kNb1 == 2 ? 4200.0 : 2500.0, kEpi, kNb1 == 2 ? 17000.0 : 9000.0);
+        consider(1, s, tiles1, kNb1 == 2 ? 4200.0 : 2500.0, kEpi1, kNb1 == 2 ? 17000.0 : 9000.0);
     }
     if (pairs)
         return splits == 1

@@ -232,12 +232,50 @@ __device__ __forceinline__ float largest(const float* v) {
 }
 
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ unsigned long long pack2(float2 a) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
+    return r;
+}
+
+__device__ __forceinline__ float2 unpack2(unsigned long long a) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+    return r;
+}
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pack2(a)), "l"(pack2(b)));
+    return unpack2(r);
+}
+
+__device__ __forceinline__ float2 sub2(float2 a, float2 b) {
+    unsigned long long r;
+    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pack2(a)), "l"(pack2(b)));
+    return unpack2(r);
+}
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pack2(a)), "l"(pack2(b)));
+    return unpack2(r);
+}
+
+__device__ __forceinline__ float2 fma2v(float2 a, float2 b, float2 c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pack2(a)), "l"(pack2(b)), "l"(pack2(c)));
+    return unpack2(r);
+}
+
 // (hi, lo) of s x0 and s x1, packed. A non-finite x makes lo NaN.
 __device__ __forceinline__ void split_pair(float x0, float x1, float s, uint32_t& hi,
                                            uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(x0 * s, x1 * s);
-    const float2 hf = __half22float2(h);
-    const __half2 l = __floats2half2_rn(fmaf(x0, s, -hf.x), fmaf(x1, s, -hf.y));
+    const float2 xs = mul2(make_float2(x0, x1), make_float2(s, s));
+    const __half2 h = __floats2half2_rn(xs.x, xs.y);
+    const float2 lf = sub2(xs, __half22float2(h));   // exact
+    const __half2 l = __floats2half2_rn(lf.x, lf.y);
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = *reinterpret_cast<const uint32_t*>(&l);
 }
@@ -477,6 +515,23 @@ __device__ __forceinline__ float2 act_slope(float v) {
         return make_float2(v * s, s + w * s * (1.0f - s) * dz2);
     } else {
         return make_float2(v, 1.0f);
+    }
+}
+
+// Two values at a time: (act, act') of v; the silu in packed arithmetic.
+template <int ACT>
+__device__ __forceinline__ void act_slope2(float2 v, float2& a, float2& slope) {
+    if constexpr (ACT == kXActSilu) {
+        const float2 one = make_float2(1.0f, 1.0f);
+        const float2 z = mul2(v, make_float2(-1.4426950408889634f, -1.4426950408889634f));
+        const float2 d = add2(make_float2(ex2(z.x), ex2(z.y)), one);
+        const float2 s = make_float2(rcp(d.x), rcp(d.y));
+        a = mul2(v, s);
+        slope = mul2(s, fma2v(v, sub2(one, s), one));
+    } else {
+        const float2 p = act_slope<ACT>(v.x), q = act_slope<ACT>(v.y);
+        a = make_float2(p.x, q.x);
+        slope = make_float2(p.y, q.y);
     }
 }
 
@@ -1038,8 +1093,12 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
                             acc[64 + j], acc[64 + j + 1], acc[64 + j + 2], acc[64 + j + 3]);
                     }
 #pragma unroll
-                    for (int e = j; e < j + 4; ++e)
-                        acc[e] = act_slope<decltype(kind)::value>(acc[e]).x * acc[64 + e];
+                    for (int e = j; e < j + 4; e += 2) {
+                        float2 ac, sl;
+                        act_slope2<decltype(kind)::value>(make_float2(acc[e], acc[e + 1]), ac, sl);
+                        const float2 h = mul2(ac, make_float2(acc[64 + e], acc[64 + e + 1]));
+                        acc[e] = h.x, acc[e + 1] = h.y;
+                    }
                 }
             });
             if (g.store_h) rowmax[half * kXBlk + row] = largest<64>(acc);
@@ -1146,12 +1205,18 @@ with_act(g.act, [&](auto kind) {
                         const float gs[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
                         const float us[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
 #pragma unroll
-                        for (int x = 0; x < 8; ++x) {
-                            const float dh = acc[b * 64 + ch * 8 + x];
-                            const float2 as = act_slope<decltype(kind)::value>(gs[x]);
-                            dg[x] = dh * us[x] * as.y;
-                            du[x] = dh * as.x;
-                            hh[x] = live ? as.x * us[x] : 0.0f;
+                        for (int x = 0; x < 8; x += 2) {
+                            const float* v = acc + b * 64 + ch * 8 + x;
+                            const float2 dh = make_float2(v[0], v[1]);
+                            const float2 u = make_float2(us[x], us[x + 1]);
+                            float2 ac, sl;
+                            act_slope2<decltype(kind)::value>(make_float2(gs[x], gs[x + 1]), ac,
+                                                              sl);
+                            const float2 p = mul2(mul2(dh, u), sl), q = mul2(dh, ac);
+                            const float2 h = mul2(ac, u);
+                            dg[x] = p.x, dg[x + 1] = p.y;
+                            du[x] = q.x, du[x + 1] = q.y;
+                            hh[x] = live ? h.x : 0.0f, hh[x + 1] = live ? h.y : 0.0f;
                         }
                         store_split8(g.o[0].data + off, half * 8 + ch0 + ch, row, dg, s0);
                         store_split8(g.o[1].data + off, half * 8 + ch0 + ch, row, du, s1);

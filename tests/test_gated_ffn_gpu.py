@@ -336,3 +336,26 @@ def test_repeated_calls_give_the_same_bits(cuda):
     for _ in range(3):
         assert all(torch.equal(a, b)
                    for a, b in zip(first, mf.gated_ffn_backward(dy, x, wg, wu, wd)))
+
+
+def test_saved_of_another_call_is_refused(cuda):
+    x, wg, wu, wd, dy = inputs(cuda, 20, 30, 40)
+    saved = mf.gated_ffn(x, wg, wu, wd, save=True)[1]
+    with pytest.raises(TypeError):
+        mf.gated_ffn_backward(dy, x, wg, wu, wd, saved=saved.buffer)
+    with pytest.raises(ValueError, match="another call"):
+        mf.gated_ffn_backward(dy[:5], x[:5], wg, wu, wd, saved=saved)
+    with pytest.raises(ValueError, match="another call"):
+        mf.gated_ffn_backward(dy, x, wg, wu, wd, "gelu", saved=saved)
+    with pytest.raises(ValueError, match="another call"):
+        mf.gated_ffn_backward(dy, x, wg, wu, wd,
+                              saved=mf.GatedSaved(saved.buffer[:8], 20, 40, "silu"))
+    with pytest.raises(ValueError, match="differs from x"):
+        mf.gated_ffn_backward(dy[:, :5], x, wg, wu, wd)
+    with pytest.raises(ValueError, match="different devices"):
+        mf.gated_ffn(x, wg.cpu(), wu, wd)
+    with pytest.raises(ValueError, match="different devices"):
+        mf.gated_ffn_backward(dy.cpu(), x, wg, wu, wd)
+    with pytest.raises(ValueError, match="different devices"):
+        mf.embedding(x, torch.zeros(3, dtype=torch.int64))
+    assert mf.device_status() == 0
