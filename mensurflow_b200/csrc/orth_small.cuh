@@ -212,13 +212,15 @@ __global__ void __launch_bounds__(kOrthThreads, 1)
             tc_fence_before();
             __syncthreads();
             product_done();
-            // g
+            // g; its rows from k on come from columns of x that no thread has written (x on its
+            // side), and would set the scale
 #pragma unroll
             for (int t = 0; t < kOrthCols / 16; ++t) {
                 float r[16];
                 if (t < gk) tmem_ld_32x32b_x16(lanes + t * 16, r);
 #pragma unroll
-                for (int j = 0; j < 16; ++j) acc[t * 16 + j] = t < gk ? (r[j] * xi) * xi : 0.0f;
+                for (int j = 0; j < 16; ++j)
+                    acc[t * 16 + j] = t < gk && row < k ? (r[j] * xi) * xi : 0.0f;
             }
             if (ranks > 1) {
                 float4* mine = reinterpret_cast<float4*>(sp) + threadIdx.x;

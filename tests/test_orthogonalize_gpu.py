@@ -140,3 +140,20 @@ def test_streams_and_graphs(cuda, shape):
         torch.cuda.synchronize()
         assert all(torch.equal(o, expect) for o in outs)
     assert mf.device_status() == 0
+
+
+@pytest.mark.parametrize("shape", [(200, 5), (1000, 40), (600, 100), (5, 200), (90, 60)])
+def test_what_ran_before_does_not_matter(cuda, shape):
+    """The same bits whatever the kernels before left in shared memory."""
+    u = torch.randn(32, *shape, device=cuda)
+    other = torch.randn(148, 128, 1024, device=cuda)
+    w = [torch.randn(*s, device=cuda) for s in ((512, 1024), (512, 1024), (1024, 512))]
+    first = mf.orthogonalize(u)
+    close(first, want(u))
+    for x in (w[2] * 1e-30, torch.full_like(w[2], 1e15), torch.full_like(w[2], float("inf"))):
+        mf.gated_ffn(x, *w)
+        assert torch.equal(mf.orthogonalize(u), first)
+    for x in (other * 1e30, other.mT):
+        mf.orthogonalize(x)
+        assert torch.equal(mf.orthogonalize(u), first)
+    assert mf.device_status() == 0
