@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(256)
         if (i >= n) break;
         const long long id = static_cast<long long>(ids[i]);
         const bool inside = id >= 0 && id < rows;
-        if (!inside && id != padding) atomicOr(&g_index_error, 1u);
+        if (!inside && (padding < 0 || id != padding)) atomicOr(&g_index_error, 1u);
         const uint32_t key = static_cast<uint32_t>(inside && id != padding ? id : rows);
         keys[i] = key;
         if (key < rows) {
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(1024, 1)
         if (i < count) {
             const long long id = static_cast<long long>(ids[first + i]);
             const bool inside = id >= 0 && id < rows;
-            if (!inside && id != padding) atomicOr(&g_index_error, 1u);
+            if (!inside && (padding < 0 || id != padding)) atomicOr(&g_index_error, 1u);
             key[r] = static_cast<uint32_t>(inside && id != padding ? id : rows);
             if (key[r] < rows) {
                 uint32_t* word = present + (key[r] >> 5);

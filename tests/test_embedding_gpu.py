@@ -138,3 +138,16 @@ def test_streams_and_graphs(cuda):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for o in outs for a, b in zip(o, expect))
     assert mf.device_status() == 0
+
+
+@pytest.mark.parametrize("tokens", [4, 70000])
+def test_minus_one_is_outside_the_table(cuda, tokens):
+    """Without a padding id -1 is an id like any other outside the table."""
+    ids = torch.arange(tokens, device=cuda) % 10
+    ids[1] = -1
+    grad = torch.randn(tokens, 8, device=cuda)
+    close(mf.embedding_grad(grad, ids, 10), grad, ids, 10, 1.0)
+    assert mf.device_status() == 0x20
+    close(mf.embedding_grad(grad, ids.int(), 10, padding=3), grad, ids, 10, 1.0, padding=3)
+    assert mf.device_status() == 0x20
+    assert mf.device_status() == 0
