@@ -342,11 +342,12 @@ int mfk_copy_peer(void* dst, int32_t dst_device, const void* src, int32_t src_de
  *     gate = x w_gate, up = x w_up, h = act(gate) * up, y = h w_down.
  * x is rows x d, w_gate and w_up d x f, w_down f x d; element (i, j) of a matrix at
  * p[i*rs + j*cs]. x_cs must be 1; of each other matrix's two strides one must be 1
- * (MFK_ERR_UNSUPPORTED otherwise; weights stored [outputs, inputs] have rs = 1). w_gate and w_up must
- * lie the same way round. activation is any mfk_activation. No counterpart in the reference, which
- * composes such blocks from gemm and elementwise calls; like mfk_gemm_f32's 3xTF32 form the
- * products are fp32-faithful: each matrix is split into fp16 (hi, lo) pairs under power-of-two
- * scales, three products are summed, and sums are held in fp32 over any depth. The rows of x and
+ * (MFK_ERR_UNSUPPORTED otherwise; weights stored [outputs, inputs] have rs = 1). w_gate and w_up
+ * must lie the same way round. rows, d and f are at most 2^30. activation is any mfk_activation.
+ * Outputs must not overlap inputs. No counterpart in the reference, which composes such blocks from
+ * gemm and elementwise calls; like mfk_gemm_f32's 3xTF32 form the products are fp32-faithful: each
+ * matrix is split into fp16 (hi, lo) pairs under power-of-two scales, three products are summed,
+ * and sums are held in fp32 over any depth. The rows of x and
  * of h have a scale each per 128 columns, so no row of y depends on another; the weights, and in
  * the backward pass every matrix, have one per 128 x 128 block. Under one scale an entry keeps 22
  * bits or more while it is within 2^-17 of the largest, and an absolute error of 2^-39 of that one
@@ -417,16 +418,16 @@ int mfk_orthogonalize_f32(const float* update, int64_t batch, int64_t rows, int6
  * id_bytes 4 or 8 (signed). No counterpart in the reference.
  *
  * mfk_embedding_f32: out[i] = scale * table[ids[i]] for the n ids; table is rows x d with row
- * stride ld (any, 0 for one row seen many times), out n x d with row stride ld_out >= d. An id outside [0, rows) gives a row of
- * zeros and sets MFK_DEVERR_INDEX in the device error word.
+ * stride ld (0 for one row seen many times), out n x d with row stride ld_out >= d. An id outside
+ * [0, rows) gives a row of zeros and sets MFK_DEVERR_INDEX in the device error word.
  *
  * mfk_embedding_grad_f32: out[v] = scale * (sum of grad[i] over the i with ids[i] == v) for every
  * v of [0, rows): a dense gradient, rows that no id names are zeros. grad is n x d with row stride
- * ld_grad (any, 0 broadcasts), out rows x d with row stride ld >= d (written, not added to). Tokens whose id is
- * `padding` take no part (-1: none is left out); an id outside [0, rows) that is not `padding`
- * takes no part either and sets MFK_DEVERR_INDEX. The sums are fp32, in an order that depends on
- * the ids and sizes alone, so repeated calls give the same bits. The workspace (16 bytes per
- * token, n d / 2 bytes at most for partial rows) comes from the stream-ordered allocator. */
+ * ld_grad (0 broadcasts), out rows x d with row stride ld >= d (written, not added to). Tokens
+ * whose id is `padding` take no part (negative: none is left out); an id outside [0, rows) that is
+ * not `padding` takes no part either and sets MFK_DEVERR_INDEX. With rows = 0 nothing is done. The
+ * sums are fp32, in an order that depends on the ids and sizes alone, so repeated calls give the
+ * same bits. The workspace (16 bytes per token, n d / 2 bytes at most for partial rows) comes from the stream-ordered allocator. */
 int mfk_embedding_f32(const float* table, int64_t rows, int64_t d, int64_t ld, const void* ids,
                       int32_t id_bytes, int64_t n, float scale, float* out, int64_t ld_out,
                       void* stream);

@@ -1,5 +1,6 @@
 """Operators of language models, on B200 tensors: the gated feed-forward block with its backward
-pass, the orthogonalised update and the embedding with its gradient, beside ``linear`` and ``linear_backward``.
+pass, the orthogonalised update and the embedding with its gradient, beside ``linear`` and
+``linear_backward``.
 
 They follow the package's manner: fp32 CUDA tensors, work queued on the current stream of the
 tensors' device, explicit backward functions, ``ValueError`` for bad arguments and
@@ -197,6 +198,7 @@ def gated_ffn_backward(grad: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor
         if not isinstance(saved, GatedSaved):
             raise TypeError(f"{op}: saved must come from gated_ffn(..., save=True)")
         if (saved.rows, saved.features) != (rows, f) or saved.buffer.device != x.device or \
+                saved.buffer.dtype is not torch.float32 or not saved.buffer.is_contiguous() or \
                 saved.buffer.numel() != _lib.lib().mfk_gated_ffn_saved_floats(rows, f) or \
                 _GATED_ACTS[saved.activation] != desc.activation:
             raise ValueError(f"{op}: saved belongs to another call ({saved.rows} rows, "
@@ -295,8 +297,8 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0) -> tor
     out = table.new_empty(ids.shape + (d,))
     if n and d:
         _run(table.device, op, _lib.lib().mfk_embedding_f32, t.data_ptr(), rows, d,
-             t.stride(0) if rows > 1 else d, index.data_ptr(), index.element_size(), n, float(scale),
-             out.data_ptr(), d)
+             t.stride(0) if rows > 1 else d, index.data_ptr(), index.element_size(), n,
+             float(scale), out.data_ptr(), d)
     return out
 
 
@@ -318,6 +320,8 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, rows: int, scale: floa
         raise ValueError(f"{op}: padding {padding} is outside the table of {rows} rows")
     _kernel_for(op, grad)
     d, n = grad.shape[-1], index.numel()
+    if rows == 0 and n and d:
+        raise ValueError(f"{op}: the table has no rows")
     g = _rows_of(grad, n, d)
     if d > 1 and g.stride(1) != 1:
         g = contiguous(g)

@@ -264,9 +264,9 @@ int x_product(XWorkspace& ws, mfk::XArgs& g, int64_t k0, int64_t k1, int64_t bat
     const int64_t tiles2 = g.sym ? tm2 * (tm2 + 1) / 2 : tm2 * tn2;
     const int64_t tiles1 = g.sym ? tm1 * (tm1 + 1) / 2 : tm1 * tn1;
     if (tiles1 * batch > (int64_t(1) << 26)) return MFK_ERR_UNSUPPORTED;
-    // What the epilogue adds to a wave, measured at 8 chunks. The backward one has three outputs and
-    // two inputs, and no registers to spare beside a pair's 128 sums a thread: 4096 x 1024 x 4096
-    // takes 163 us by pairs and 154 by single CTAs (at 32 chunks the pairs win).
+    // What the epilogue adds to a wave, measured at 8 chunks. The backward one has three outputs
+    // and two inputs, and no registers to spare beside a pair's 128 sums a thread: 4096 x 1024 x
+    // 4096 takes 163 us by pairs and 154 by single CTAs (at 32 chunks the pairs win).
     constexpr double kEpi1 = EPI == mfk::kXGatedBwd ? 10000.0 : EPI == mfk::kXGated ? 7000.0
                                                                                     : 3000.0;
     constexpr double kEpi2 = EPI == mfk::kXGatedBwd ? 30000.0 : EPI == mfk::kXGated ? 7000.0
@@ -322,7 +322,7 @@ namespace {
 
 // ---- the gated feed-forward block ------------------------------------------------------------
 
-constexpr int64_t kXMaxDim = (int64_t(1) << 31) - 256;
+constexpr int64_t kXMaxDim = int64_t(1) << 30;  // 32-bit indexes may run a few tiles further
 
 int check_gated(const mfk_gated_ffn_desc* d) {
     if (d == nullptr) return MFK_ERR_INVALID_ARGUMENT;
@@ -660,8 +660,9 @@ int run_orthogonalize(const float* u, int64_t batch, int64_t rows, int64_t cols,
             rc = x_product<mfk::kXSplit>(ws, g, k, 0, batch);
             if (rc != MFK_OK) return rc;
         }
-        // x = ca x + poly x (or x poly). (With ca on poly's diagonal no third matrix is read, but then
-        // the largest term is rounded toward zero with the rest: 2.2e-6 off after five steps, not 8e-7.)
+        // x = ca x + poly x (or x poly). (With ca on poly's diagonal no third matrix is read, but
+        // then the largest term is rounded toward zero with the rest: 2.2e-6 off after five steps,
+        // not 8e-7.)
         mfk::XArgs g{};
         if (tall) {
             g.a[0] = g.a[1] = x_operand(ws, *x, true);

@@ -6,7 +6,8 @@
 //     hi = fp16(s x),  lo = fp16(s x - hi),
 // so s x = hi + lo to 2^-23 of itself (and never worse than 2^-40 of the block's largest entry:
 // lo's spacing ends at 2^-24). An operand whose rows are the result's rows may have one s per row
-// of a block instead (`by_row`): then no row's accuracy depends on another's size. A product of two such matrices takes three fp16 products,
+// of a block instead (`by_row`): then no row's accuracy depends on another's size. A product of two
+// such matrices takes three fp16 products,
 //     (s_a a)(s_b b) ~ lo hi + hi lo + hi hi,
 // summed in fp32; the term left out, lo lo, is below 2^-22 of the product. fp16 tensor products
 // run at twice the tf32 rate, so this is twice as fast as a tf32 three-way split of the same 22
@@ -14,10 +15,10 @@
 //
 // Accumulation. tcgen05 rounds its fp32 accumulator toward zero on every instruction: each one
 // loses about 3.4e-8 of the running sum, always towards zero (measured: 3.8e-6 relative to the
-// result after 192 instructions, 1.2e-5 after 3072 spread over stream-K parts). So a tensor-memory accumulator
-// only ever holds one 128-deep chunk (24 instructions, the small lo products of a stage first),
-// and the epilogue warps add the chunks, scaled by the two blocks' 1/s, in fp32 registers with
-// round to nearest.
+// result after 192 instructions, 1.2e-5 after 3072 spread over stream-K parts). So a tensor-memory
+// accumulator only ever holds one 128-deep chunk (24 instructions, the small lo products of a stage
+// first), and the epilogue warps add the chunks, scaled by the two blocks' 1/s, in fp32 registers
+// with round to nearest.
 //
 // Layout. A block is 64 KB: hi then lo, each as 16 columns-of-eight ("lines"), a line holding
 // 128 rows x 8 halves (16 bytes a row, 2 KB). 8 rows x 16 bytes are one core matrix of the
@@ -230,7 +231,6 @@ __device__ __forceinline__ float largest(const float* v) {
     }
     return m;
 }
-
 
 // Two fp32 operations in one instruction.
 __device__ __forceinline__ unsigned long long pack2(float2 a) {
@@ -479,7 +479,8 @@ __device__ __forceinline__ float logistic(float z) {
 // act(v) and act'(v) in fp32. silu and the tanh form of GELU go through the logistic function s:
 // 0.5 (1 + tanh z) = s(2 z). The kind is a template parameter and the epilogues branch on it once
 // per tile: with the branch inside the unrolled loops the code of all kinds lies between one
-// element and the next, and fetching it took three quarters of the kernel's time.
+// element and the next, and fetching it took half of the kernels' time (4096 x 1024 x 4096: forward
+// 380 us, 192 without it; backward 435 and 190).
 template <int ACT>
 __device__ __forceinline__ float2 act_slope(float v) {
     if constexpr (ACT == kXActSilu) {
@@ -770,9 +771,9 @@ __device__ __forceinline__ void x_max_into(uint32_t* red, float amax) {
 //
 // SPL: the contraction is shared by g.splits CTAs (or pairs) of one cluster, one tile each. A CTA
 // leaves its sums in its own shared memory (the stages are read by then) and takes over its share
-// of each thread's eight groups of eight columns (at most four): it adds the cluster's sums of those, in rank order,
-// through distributed shared memory, and finishes them. (Through L2, with one CTA adding and
-// finishing everything, the exchange took 8 us of a 17 us product.)
+// of each thread's eight groups of eight columns (at most four): it adds the cluster's sums of
+// those, in rank order, through distributed shared memory, and finishes them. (Through L2, with one
+// CTA adding and finishing everything, the exchange took 8 us of a 17 us product.)
 template <int CG, int NB, int EPI, bool SPL>
 __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint8_t* epi_smem,
                                            uint32_t* red, uint32_t tmem, uint64_t* tfull,
@@ -1190,38 +1191,39 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
                         g.o[2].inv[blk] = i2;
                     }
                     const long long off = static_cast<long long>(blk) * kXBlockBytes;
-with_act(g.act, [&](auto kind) {
+                    with_act(g.act, [&](auto kind) {
 #pragma unroll
-                    for (int ch = 0; ch < 8; ++ch) {
-                        if (SPL && ch >= ng) break;
-                        float dg[8], du[8], hh[8];
-                        const int turn = b * ng + ch;
-                        const uint32_t src =
-                            smem_u32(box) + (turn % kSlots) * (4096 / kSlots) + lane * 16;
-                        cp_async_wait<kSlots - 1>();
-                        const float4 g0 = ld_shared_v4(src), g1 = ld_shared_v4(src + 512);
-                        const float4 u0 = ld_shared_v4(src + 1024), u1 = ld_shared_v4(src + 1536);
-                        fetch(turn + kSlots);
-                        const float gs[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
-                        const float us[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
+                        for (int ch = 0; ch < 8; ++ch) {
+                            if (SPL && ch >= ng) break;
+                            float dg[8], du[8], hh[8];
+                            const int turn = b * ng + ch;
+                            const uint32_t src =
+                                smem_u32(box) + (turn % kSlots) * (4096 / kSlots) + lane * 16;
+                            cp_async_wait<kSlots - 1>();
+                            const float4 g0 = ld_shared_v4(src), g1 = ld_shared_v4(src + 512);
+                            const float4 u0 = ld_shared_v4(src + 1024);
+                            const float4 u1 = ld_shared_v4(src + 1536);
+                            fetch(turn + kSlots);
+                            const float gs[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
+                            const float us[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
 #pragma unroll
-                        for (int x = 0; x < 8; x += 2) {
-                            const float* v = acc + b * 64 + ch * 8 + x;
-                            const float2 dh = make_float2(v[0], v[1]);
-                            const float2 u = make_float2(us[x], us[x + 1]);
-                            float2 ac, sl;
-                            act_slope2<decltype(kind)::value>(make_float2(gs[x], gs[x + 1]), ac,
-                                                              sl);
-                            const float2 p = mul2(mul2(dh, u), sl), q = mul2(dh, ac);
-                            const float2 h = mul2(ac, u);
-                            dg[x] = p.x, dg[x + 1] = p.y;
-                            du[x] = q.x, du[x + 1] = q.y;
-                            hh[x] = live ? h.x : 0.0f, hh[x + 1] = live ? h.y : 0.0f;
+                            for (int x = 0; x < 8; x += 2) {
+                                const float* v = acc + b * 64 + ch * 8 + x;
+                                const float2 dh = make_float2(v[0], v[1]);
+                                const float2 u = make_float2(us[x], us[x + 1]);
+                                float2 ac, sl;
+                                act_slope2<decltype(kind)::value>(make_float2(gs[x], gs[x + 1]), ac,
+                                                                  sl);
+                                const float2 p = mul2(mul2(dh, u), sl), q = mul2(dh, ac);
+                                const float2 h = mul2(ac, u);
+                                dg[x] = p.x, dg[x + 1] = p.y;
+                                du[x] = q.x, du[x + 1] = q.y;
+                                hh[x] = live ? h.x : 0.0f, hh[x + 1] = live ? h.y : 0.0f;
+                            }
+                            store_split8(g.o[0].data + off, half * 8 + ch0 + ch, row, dg, s0);
+                            store_split8(g.o[1].data + off, half * 8 + ch0 + ch, row, du, s1);
+                            store_split8(g.o[2].data + off, half * 8 + ch0 + ch, row, hh, s2);
                         }
-                        store_split8(g.o[0].data + off, half * 8 + ch0 + ch, row, dg, s0);
-                        store_split8(g.o[1].data + off, half * 8 + ch0 + ch, row, du, s1);
-                        store_split8(g.o[2].data + off, half * 8 + ch0 + ch, row, hh, s2);
-                    }
                     });
                 }
             }

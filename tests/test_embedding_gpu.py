@@ -151,3 +151,11 @@ def test_minus_one_is_outside_the_table(cuda, tokens):
     close(mf.embedding_grad(grad, ids.int(), 10, padding=3), grad, ids, 10, 1.0, padding=3)
     assert mf.device_status() == 0x20
     assert mf.device_status() == 0
+
+
+def test_a_table_without_rows(cuda):
+    ids = torch.zeros(3, dtype=torch.int64, device=cuda)
+    with pytest.raises(ValueError, match="no rows"):
+        mf.embedding(torch.empty(0, 4, device=cuda), ids)
+    with pytest.raises(ValueError, match="no rows"):
+        mf.embedding_grad(torch.zeros(3, 4, device=cuda), ids, 0)
