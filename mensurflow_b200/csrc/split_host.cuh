@@ -5,7 +5,7 @@
 
 namespace {
 
-constexpr int kXKinds = 48;  // kernel instantiations (and cluster sizes) with per-device set-up
+constexpr int kXKinds = 60;  // kernel instantiations (and cluster sizes) with per-device set-up
 
 struct XDevice {
     bool ready[kXKinds] = {};
@@ -250,7 +250,8 @@ int x_launch(XWorkspace& ws, mfk::XArgs& g, int slots, int64_t batch, int64_t tm
     return MFK_OK;
 }
 
-// Launches out[mb x nb blocks] = A B over kc0 (+ kc1) chunks. k0, k1: the segments' depths.
+// Launches out[mb x nb blocks] = A B over kc0 (+ kc1) chunks. k0, k1: the segments' depths. The third
+// product of kXWeights has the others' blocks, or those of their transposes: as many tiles.
 template <int EPI>
 int x_product(XWorkspace& ws, mfk::XArgs& g, int64_t k0, int64_t k1, int64_t batch) {
     constexpr int kNb1 = EPI == mfk::kXGated ? 2 : 1;  // the one-CTA kernel's blocks per tile
@@ -298,6 +299,8 @@ int x_product(XWorkspace& ws, mfk::XArgs& g, int64_t k0, int64_t k1, int64_t bat
         if (rc != MFK_OK) return rc;
         consider(1, s, tiles1, kNb1 == 2 ? 4200.0 : 2500.0, kEpi1, kNb1 == 2 ? 17000.0 : 9000.0);
     }
+    g.third.tiles_m = pairs ? (g.third.mb + 1) / 2 : g.third.mb;
+    g.third.tiles_n = pairs ? (g.third.nb + 1) / 2 : g.third.nb;
     if (pairs)
         return splits == 1
                    ? x_launch<2, 2, EPI, false>(ws, g, best_slots, batch, tm2, tn2, tiles2, 1)
@@ -413,26 +416,38 @@ int run_gated_ffn(const mfk_gated_ffn_desc* d, float* y, int64_t ldy, float* sav
     return x_product<mfk::kXF32>(ws, g, d->f, 0, 1);
 }
 
-// out (rows x cols, strides rs / cs of which one is 1) = sum over the stored rows of a and b:
-// a^T b, or its transpose with the operands exchanged where `out` is column-major.
-int x_weight_grad(XWorkspace& ws, const XMat& a, const XMat& b, int64_t rows, int64_t cols,
-                  int64_t depth, float* out, int64_t rs, int64_t cs, int64_t batch, int64_t out_bs,
-                  bool batch_in_a) {
-    bool t = false;
-    if (!x_orientation(rows, cols, rs, cs, &t)) return MFK_ERR_UNSUPPORTED;
-    mfk::XOperand oa = x_operand(ws, a, false), ob = x_operand(ws, b, false);
-    if (batch > 1) (batch_in_a ? oa : ob).bstride = static_cast<int>((batch_in_a ? a : b).blocks());
+// The weights' gradients in one launch, so that the last tiles of one run beside the first of the
+// next: (dw_gate, dw_up) = x^T (dgate, dup) and dw_down = h^T dy, all over the rows. A column-major
+// result is the transposed product with the operands exchanged. (1531 rows, 1003 x 2731: 88 and 44
+// tiles on 74 pairs are three waves, 132 are two.)
+int x_weight_grads(XWorkspace& ws, const mfk_gated_ffn_desc* d, const mfk_gated_ffn_grads* o,
+                   const XMat& x, const XMat& dg, const XMat& h, const XMat& dy) {
+    bool t = false, td = false;
+    if (!x_orientation(d->d, d->f, o->dw_rs, o->dw_cs, &t) ||
+        !x_orientation(d->f, d->d, o->dw_down_rs, o->dw_down_cs, &td))
+        return MFK_ERR_UNSUPPORTED;
+    mfk::XOperand ox = x_operand(ws, x, false), odg = x_operand(ws, dg, false);
+    const mfk::XOperand oh = x_operand(ws, h, false), ody = x_operand(ws, dy, false);
+    odg.bstride = static_cast<int>(dg.blocks());   // dup lies behind dgate
     mfk::XArgs g{};
-    g.a[0] = g.a[1] = t ? ob : oa;
-    g.b[0] = g.b[1] = t ? oa : ob;
-    g.m = static_cast<int>(t ? cols : rows);
-    g.n = static_cast<int>(t ? rows : cols);
+    g.a[0] = t ? odg : ox;
+    g.b[0] = t ? ox : odg;
+    g.m = static_cast<int>(t ? d->f : d->d);
+    g.n = static_cast<int>(t ? d->d : d->f);
     g.mb = (g.m + 127) / 128;
     g.nb = (g.n + 127) / 128;
-    g.out = out;
-    g.ld = t ? cs : rs;
-    g.out_bs = out_bs;
-    return x_product<mfk::kXF32>(ws, g, depth, 0, batch);
+    g.out = o->dw_gate;
+    g.ld = t ? o->dw_cs : o->dw_rs;
+    g.out_bs = o->dw_up - o->dw_gate;
+    g.a[1] = td ? ody : oh;
+    g.b[1] = td ? oh : ody;
+    g.third.m = static_cast<int>(td ? d->d : d->f);
+    g.third.n = static_cast<int>(td ? d->f : d->d);
+    g.third.mb = (g.third.m + 127) / 128;
+    g.third.nb = (g.third.n + 127) / 128;
+    g.third.out = o->dw_down;
+    g.third.ld = td ? o->dw_down_cs : o->dw_down_rs;
+    return x_product<mfk::kXWeights>(ws, g, d->rows, 0, 3);
 }
 
 int run_gated_ffn_backward(const mfk_gated_ffn_desc* d, const mfk_gated_ffn_grads* o,
@@ -540,14 +555,7 @@ int run_gated_ffn_backward(const mfk_gated_ffn_desc* d, const mfk_gated_ffn_grad
         rc = x_product<mfk::kXF32>(ws, g, d->f, d->f, 1);
         if (rc != MFK_OK) return rc;
     }
-    if (need_w) {  // (dw_gate, dw_up) = x^T (dgate, dup), dw_down = h^T dy
-        rc = x_weight_grad(ws, x, dg, d->d, d->f, d->rows, o->dw_gate, o->dw_rs, o->dw_cs, 2,
-                           o->dw_up - o->dw_gate, false);
-        if (rc != MFK_OK) return rc;
-        rc = x_weight_grad(ws, h, dy, d->f, d->d, d->rows, o->dw_down, o->dw_down_rs,
-                           o->dw_down_cs, 1, 0, false);
-        if (rc != MFK_OK) return rc;
-    }
+    if (need_w) return x_weight_grads(ws, d, o, x, dg, h, dy);
     return MFK_OK;
 }
 

@@ -45,7 +45,14 @@ constexpr int kXEpiWarp0 = 2;
 constexpr int kXEpiThreads = 256;
 constexpr int kXBoxFloats = 32 * 32;
 
-enum XEpi : int { kXF32 = 0, kXSplit = 1, kXGated = 2, kXGatedBwd = 3 };
+// kXWeights: fp32 results of three products in one launch, two of one shape (a batch) and a third
+// with sizes and operands of its own over the same depth.
+enum XEpi : int { kXF32 = 0, kXSplit = 1, kXGated = 2, kXGatedBwd = 3, kXWeights = 4 };
+
+template <int EPI>
+__host__ __device__ constexpr bool x_fp32() {
+    return EPI == kXF32 || EPI == kXWeights;
+}
 
 // A split matrix as an operand: block (mn, k) of matrix z.
 struct XOperand {
@@ -65,7 +72,8 @@ struct XOut {
 };
 
 struct XArgs {
-    XOperand a[2], b[2];   // two segments of the contraction, or (gated) b = gate and up
+    XOperand a[2], b[2];   // two segments of the contraction, or (gated) b = gate and up, or
+                           // (weights) the batch's and the third product's
     int kc0, kc;           // chunks of 128 in segment 0, in all
     int last0, last1;      // stages of 64 in each segment's last chunk (1 or 2)
     int mb, nb;            // output blocks
@@ -76,6 +84,11 @@ struct XArgs {
     XOut c;                // C as a split matrix (beta != 0)
     float* out;            // fp32 output, row stride ld, batch stride out_bs
     long long ld, out_bs;
+    struct {               // the third product of kXWeights
+        int tiles_m, tiles_n, mb, nb, m, n;
+        float* out;
+        long long ld;
+    } third;
     XOut o[3];             // split outputs: result / h; dgate, dup, h
     float* gate;           // saved pre-activations in accumulator order (null: not saved)
     float* up;
@@ -568,6 +581,12 @@ struct XUnit {
     int z, tm, tn, s, c0, c1, tile;
 };
 
+template <int EPI>
+__device__ __forceinline__ bool x_third(int z) {
+    return EPI == kXWeights && z == 2;
+}
+
+template <int EPI>
 __device__ __forceinline__ XUnit x_unit(const XArgs& g, int u) {
     XUnit w;
     const int t = u / g.splits;
@@ -582,10 +601,12 @@ __device__ __forceinline__ XUnit x_unit(const XArgs& g, int u) {
         w.tm = i;
         w.tn = q - i * (i + 1) / 2;
     } else {  // bands of eight tile rows, column by column, so the operands in flight stay in L2
-        const int band = q / (8 * g.tiles_n);
+        const int tiles_m = x_third<EPI>(w.z) ? g.third.tiles_m : g.tiles_m;
+        const int tiles_n = x_third<EPI>(w.z) ? g.third.tiles_n : g.tiles_n;
+        const int band = q / (8 * tiles_n);
         const int first = band * 8;
-        const int height = min(8, g.tiles_m - first);
-        q -= first * g.tiles_n;
+        const int height = min(8, tiles_m - first);
+        q -= first * tiles_n;
         w.tn = q / height;
         w.tm = first + q - w.tn * height;
     }
@@ -635,11 +656,13 @@ __device__ __forceinline__ void x_producer(const XArgs& g, const CUtensorMap* mk
     int stage = 0;
     uint32_t phase = 0;
     for (int u = first; u < g.units; u += step) {
-        const XUnit w = x_unit(g, u);
-        const int i = min(w.tm * CG + static_cast<int>(rank), g.mb - 1);
+        const XUnit w = x_unit<EPI>(g, u);
+        const int nb = x_third<EPI>(w.z) ? g.third.nb : g.nb;
+        const int i = min(w.tm * CG + static_cast<int>(rank),
+                          (x_third<EPI>(w.z) ? g.third.mb : g.mb) - 1);
         for (int c = w.c0; c < w.c1; ++c) {
-            const int seg = EPI == kXF32 && c >= g.kc0 ? 1 : 0;
-            const int k = seg ? c - g.kc0 : c;
+            const int seg = x_third<EPI>(w.z) || (EPI == kXF32 && c >= g.kc0) ? 1 : 0;
+            const int k = EPI == kXF32 && seg ? c - g.kc0 : c;
             const int halves = c == g.kc0 - 1 ? g.last0 : (c == g.kc - 1 ? g.last1 : 2);
             for (int h = 0; h < halves; ++h) {
                 if (!mbar_wait(&empty[stage], phase ^ 1u, 1u << 0)) {
@@ -667,7 +690,7 @@ __device__ __forceinline__ void x_producer(const XArgs& g, const CUtensorMap* mk
                                    w.tn, w.tn, k, h);
                     } else {
                         x_load<CG>(s + 32768 * (1 + b), mk, mm, &full[stage], bar0, g.b[seg], w.z,
-                                   w.tn * NB, min(w.tn * NB + bb, g.nb - 1), k, h);
+                                   w.tn * NB, min(w.tn * NB + bb, nb - 1), k, h);
                     }
                 }
                 if (++stage == C::kStages) {
@@ -691,11 +714,11 @@ __device__ __forceinline__ void x_mma(const XArgs& g, uint32_t tmem, uint8_t* st
     uint32_t phase = 0, tphase = 0;
     const uint32_t stage0 = smem_u32(stages);
     for (int u = first; u < g.units; u += step) {
-        const XUnit w = x_unit(g, u);
+        const XUnit w = x_unit<EPI>(g, u);
         const int i = w.tm * CG, j = EPI == kXGated ? w.tn : w.tn * NB;
         for (int c = w.c0; c < w.c1; ++c) {
-            const int seg = EPI == kXF32 && c >= g.kc0 ? 1 : 0;
-            const int k = seg ? c - g.kc0 : c;
+            const int seg = x_third<EPI>(w.z) || (EPI == kXF32 && c >= g.kc0) ? 1 : 0;
+            const int k = EPI == kXF32 && seg ? c - g.kc0 : c;
             const int halves = c == g.kc0 - 1 ? g.last0 : (c == g.kc - 1 ? g.last1 : 2);
             const int fa = x_flip(g.a[seg], i, k), fb = x_flip(g.b[seg], j, k);
             // K-major: core matrices 2 KB apart along k, 128 B along rows; 16 deep = two lines.
@@ -789,9 +812,11 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
     uint32_t tphase = 0;
     bool alive = true;  // a wait that gave up: finish without waiting, so every barrier is met
     for (int u = first; u < g.units; u += step) {
-        const XUnit w = x_unit(g, u);
+        const XUnit w = x_unit<EPI>(g, u);
         const int i = w.tm * CG + static_cast<int>(rank);
-        const int i_in = min(i, g.mb - 1);
+        const bool third = x_third<EPI>(w.z);
+        const int mb = third ? g.third.mb : g.mb, nb = third ? g.third.nb : g.nb;
+        const int i_in = min(i, mb - 1);
         // this CTA's groups of eight columns: ng of them from ch0
         const int ch0 = SPL ? 8 * w.s / g.splits : 0;
         const int ng = SPL ? 8 * (w.s + 1) / g.splits - ch0 : 8;
@@ -800,7 +825,8 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
         // slots, a split C in four. The first turns while the product is still computed (C read
         // when it was needed made the tail of a 1024 x 4096 product 6 us instead of 4).
         constexpr int kSlots = EPI == kXGatedBwd ? 2 : 4;
-        const bool reads = EPI == kXGatedBwd || (EPI != kXGated && g.beta != 0.0f);
+        const bool reads =
+            EPI == kXGatedBwd || ((EPI == kXF32 || EPI == kXSplit) && g.beta != 0.0f);
         const int turns = reads && i < g.mb ? min(NB, g.nb - w.tn * NB) * ng : 0;
         auto fetch = [&](int turn) {
             if (turn < turns) {
@@ -845,8 +871,8 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
 #pragma unroll
         for (int j = 0; j < NB * 64; ++j) acc[j] = 0.0f;
         for (int c = w.c0; c < w.c1; ++c) {
-            const int seg = EPI == kXF32 && c >= g.kc0 ? 1 : 0;
-            const int k = seg ? c - g.kc0 : c;
+            const int seg = x_third<EPI>(w.z) || (EPI == kXF32 && c >= g.kc0) ? 1 : 0;
+            const int k = EPI == kXF32 && seg ? c - g.kc0 : c;
             const int a_blk = x_block(g.a[seg], w.z, i_in, k, x_flip(g.a[seg], w.tm * CG, k));
             const float ia = g.a[seg].by_row
                                  ? g.a[seg].inv[static_cast<long long>(a_blk) * kXBlk + row]
@@ -857,7 +883,7 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
             for (int b = 0; b < NB; ++b) {
                 const XOperand& ob = EPI == kXGated ? g.b[b] : g.b[seg];
                 const int j0 = EPI == kXGated ? w.tn : w.tn * NB;
-                const int j = EPI == kXGated ? w.tn : min(j0 + b, g.nb - 1);
+                const int j = EPI == kXGated ? w.tn : min(j0 + b, nb - 1);
                 const float ib = ob.inv[x_block(ob, w.z, j, k, x_flip(ob, j0, k))];
                 f1[b] = fminf(ia, ib);  // else the smaller first: no overflow on the way
                 f2[b] = fmaxf(ia, ib);
@@ -927,7 +953,10 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
                 }
             }
         }
-        const bool row_block = i < g.mb;
+        const bool row_block = i < mb;
+        const int m = third ? g.third.m : g.m, n = third ? g.third.n : g.n;
+        float* const out = third ? g.third.out : g.out + w.z * g.out_bs;
+        const long long ld = third ? g.third.ld : g.ld;
 
         if constexpr (EPI == kXF32 || EPI == kXSplit) {
             if (reads) {  // alpha acc + beta C
@@ -964,34 +993,32 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
             }
         }
 
-        if constexpr (EPI == kXF32 && SPL) {
+        if constexpr (x_fp32<EPI>() && SPL) {
             const int grow = i * kXBlk + row;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
 #pragma unroll
                 for (int ch = 0; ch < 4; ++ch) {
                     const int col = (w.tn * NB + b) * kXBlk + half * 64 + (ch0 + ch) * 8;
-                    if (ch < ng && grow < g.m) {
-                        float* dst = g.out + w.z * g.out_bs +
-                                     static_cast<long long>(grow) * g.ld + col;
+                    if (ch < ng && grow < m) {
+                        float* dst = out + static_cast<long long>(grow) * ld + col;
                         const float* v = acc + b * 64 + ch * 8;
-                        if (col + 8 <= g.n && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
+                        if (col + 8 <= n && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
                             *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
                             *reinterpret_cast<float4*>(dst + 4) =
                                 make_float4(v[4], v[5], v[6], v[7]);
                         } else {
 #pragma unroll
                             for (int e = 0; e < 8; ++e)
-                                if (col + e < g.n) dst[e] = v[e];
+                                if (col + e < n) dst[e] = v[e];
                         }
                     }
                 }
             }
-        } else if constexpr (EPI == kXF32) {
+        } else if constexpr (x_fp32<EPI>()) {
             // through a 32 x 32 box (16-byte column group c of row r at c ^ (r % 8): no bank
             // conflicts either way), so that eight lanes write 128 bytes of a row
-            const bool wide = ((reinterpret_cast<uintptr_t>(g.out) & 15u) == 0) &&
-                              (g.ld & 3) == 0 && (g.out_bs & 3) == 0;
+            const bool wide = ((reinterpret_cast<uintptr_t>(out) & 15u) == 0) && (ld & 3) == 0;
             const uint32_t box0 = smem_u32(box);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -1007,23 +1034,22 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
                     __syncwarp();
                     const int col = (w.tn * NB + b) * kXBlk + half * 64 + t * 32 + (lane & 7) * 4;
                     const int row0 = i * kXBlk + q * 32 + (lane >> 3);
-                    if (row_block && col < g.n) {
-                        float* dst = g.out + w.z * g.out_bs + static_cast<long long>(row0) * g.ld +
-                                     col;
-                        const long long step = 4 * g.ld;
+                    if (row_block && col < n) {
+                        float* dst = out + static_cast<long long>(row0) * ld + col;
+                        const long long step = 4 * ld;
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             const int r = e * 4 + (lane >> 3);
                             const float4 v =
                                 ld_shared_v4(box0 + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-                            if (row0 + e * 4 < g.m) {
-                                if (wide && col + 4 <= g.n) {
+                            if (row0 + e * 4 < m) {
+                                if (wide && col + 4 <= n) {
                                     *reinterpret_cast<float4*>(dst) = v;
                                 } else {
                                     dst[0] = v.x;
-                                    if (col + 1 < g.n) dst[1] = v.y;
-                                    if (col + 2 < g.n) dst[2] = v.z;
-                                    if (col + 3 < g.n) dst[3] = v.w;
+                                    if (col + 1 < n) dst[1] = v.y;
+                                    if (col + 2 < n) dst[2] = v.z;
+                                    if (col + 3 < n) dst[3] = v.w;
                                 }
                             }
                             dst += step;
@@ -1251,7 +1277,7 @@ __global__ void __launch_bounds__(kXThreads, 1)
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain + 1);
     uint32_t* red = tmem_holder + 1;                       // three sets of eight block maxima
     // the cluster barriers that the epilogue warps of an SPL kernel meet at
-    constexpr int kSplitSyncs = !SPL ? 0 : EPI == kXF32 ? 2 : 3;
+    constexpr int kSplitSyncs = !SPL ? 0 : x_fp32<EPI>() ? 2 : 3;
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     // CTAs 2 p and 2 p + 1 of a cluster are a pair

@@ -7,11 +7,14 @@ the chunks then add in fp32, 2^-24 each. So an entry is off by TOL |A||B| with
 TOL = 3.5e-6 + chunks * 6e-8, plus 2^-39 of a block's largest entry per operand entry (1e-11
 relative to it, included in the constant for the distributions here). The activation adds a few
 fp32 roundings (8 ulp, 1e-6). Bounds of later products are propagated through their factors."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 
 import mensurflow_b200 as mf
+from mensurflow_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -358,4 +361,38 @@ def test_saved_of_another_call_is_refused(cuda):
         mf.gated_ffn_backward(dy.cpu(), x, wg, wu, wd)
     with pytest.raises(ValueError, match="different devices"):
         mf.embedding(x, torch.zeros(3, dtype=torch.int64))
+    assert mf.device_status() == 0
+
+
+@pytest.mark.parametrize("shape", [(300, 140, 600), (17, 520, 130), (1300, 260, 900)])
+@pytest.mark.parametrize("down_transposed", [False, True])
+@pytest.mark.parametrize("transposed", [False, True])
+def test_layouts_of_the_weight_gradients(cuda, shape, transposed, down_transposed):
+    """Each weight gradient row-major or column-major, with a row stride of its own, in guarded
+    memory: what lies between the rows stays."""
+    rows, d, f = shape
+    x, wg, wu, wd, dy = inputs(cuda, rows, d, f)
+    ref = mf.gated_ffn_backward(dy, x, wg, wu, wd, need_x=False)[1:]
+    pad = 5
+
+    def guarded(r, c, t):
+        base = torch.full((c, r + pad) if t else (r, c + pad), -7.0, device=cuda)
+        return base, (base[:, :r].t() if t else base[:, :c])
+
+    outs = [guarded(d, f, transposed), guarded(d, f, transposed), guarded(f, d, down_transposed)]
+    desc = _lib.GatedFfnDesc(x.data_ptr(), d, 1, wg.data_ptr(), f, 1, wu.data_ptr(), f, 1,
+                             wd.data_ptr(), d, 1, rows, d, f, _lib.ACT_SILU, 0)
+    o = _lib.GatedFfnGrads()
+    o.grad, o.grad_rs, o.grad_cs = dy.data_ptr(), d, 1
+    o.dw_gate, o.dw_up, o.dw_down = (b.data_ptr() for b, _ in outs)
+    o.dw_rs, o.dw_cs = outs[0][1].stride()
+    o.dw_down_rs, o.dw_down_cs = outs[2][1].stride()
+    assert _lib.lib().mfk_gated_ffn_backward_f32(
+        ctypes.byref(desc), ctypes.byref(o), None,
+        ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+    for (base, view), expect in zip(outs, ref):
+        # another operand order adds the same terms in another order
+        scale = expect.abs().max()
+        assert float((view - expect).abs().max()) <= 2 * tol(rows) * 8 * float(scale)
+        assert bool((base[:, -pad:] == -7.0).all())
     assert mf.device_status() == 0
