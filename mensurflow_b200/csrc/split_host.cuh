@@ -141,9 +141,17 @@ int x_split(XWorkspace& ws, mfk::XSources& list, const XMat* const* mats, bool s
         at += mats[i]->blocks() * mats[i]->batch;
     }
     if (at == 0) return MFK_OK;
-    mfk::split_blocks_kernel<<<static_cast<unsigned>(at), 256, 0, ws.stream>>>(list);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3(static_cast<unsigned>(at), 1, 1);
+    cfg.blockDim = dim3(256, 1, 1);
+    cfg.stream = ws.stream;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = list.s[0].live != nullptr ? 1 : 0;  // beside the launch that finds the live rows
+    MFK_CUDA(cudaLaunchKernelEx(&cfg, mfk::split_blocks_kernel, list));
     g_launches.fetch_add(1);
-    MFK_CUDA(cudaGetLastError());
     return MFK_OK;
 }
 
@@ -250,8 +258,8 @@ int x_launch(XWorkspace& ws, mfk::XArgs& g, int slots, int64_t batch, int64_t tm
     return MFK_OK;
 }
 
-// Launches out[mb x nb blocks] = A B over kc0 (+ kc1) chunks. k0, k1: the segments' depths. The third
-// product of kXWeights has the others' blocks, or those of their transposes: as many tiles.
+// Launches out[mb x nb blocks] = A B over kc0 (+ kc1) chunks. k0, k1: the segments' depths. The
+// third product of kXWeights has the others' blocks, or those of their transposes: as many tiles.
 template <int EPI>
 int x_product(XWorkspace& ws, mfk::XArgs& g, int64_t k0, int64_t k1, int64_t batch) {
     constexpr int kNb1 = EPI == mfk::kXGated ? 2 : 1;  // the one-CTA kernel's blocks per tile

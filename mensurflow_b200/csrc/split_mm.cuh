@@ -345,6 +345,9 @@ __global__ void __launch_bounds__(256) split_blocks_kernel(const __grid_constant
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int r8 = lane >> 2, c4 = lane & 3;
     const float* base = t.src + z * t.bs;
+    // only the blocks that leave rows out read what the launch before writes (and with them the
+    // whole launch ends after that one)
+    if (t.live != nullptr) grid_wait();
     float v[2][4][8];
     if (t.vec) {
 #pragma unroll
