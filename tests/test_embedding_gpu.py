@@ -159,3 +159,21 @@ def test_a_table_without_rows(cuda):
         mf.embedding(torch.empty(0, 4, device=cuda), ids)
     with pytest.raises(ValueError, match="no rows"):
         mf.embedding_grad(torch.zeros(3, 4, device=cuda), ids, 0)
+
+
+def test_offsets_past_32_bits(cuda):
+    """A table of more than 2^31 entries, and its gradient."""
+    if torch.cuda.mem_get_info()[0] < 40e9:
+        pytest.skip("needs 40 GB")
+    rows, d = 2 ** 16 + 9, 2 ** 15 + 4
+    table = torch.empty(rows, d, device=cuda)
+    table.normal_()
+    ids = torch.tensor([rows - 1, 0, rows - 1, 2 ** 16], device=cuda)
+    assert torch.equal(mf.embedding(table, ids), table[ids])
+    grad = torch.randn(4, d, device=cuda)
+    out = mf.embedding_grad(grad, ids, rows)
+    assert torch.equal(out[2 ** 16], grad[3]) and torch.equal(out[0], grad[1])
+    assert torch.equal(out[rows - 1], grad[0] + grad[2])
+    out[ids] = 0.0
+    assert not out.any()
+    assert mf.device_status() == 0

@@ -396,3 +396,28 @@ def test_layouts_of_the_weight_gradients(cuda, shape, transposed, down_transpose
         assert float((view - expect).abs().max()) <= 2 * tol(rows) * 8 * float(scale)
         assert bool((base[:, -pad:] == -7.0).all())
     assert mf.device_status() == 0
+
+
+def test_offsets_past_32_bits(cuda):
+    """x, y and the gradients of more than 2^31 entries: the last rows against 64 bits. (The same
+    rows alone share their contractions among clusters: other sums, other last bits.)"""
+    d, f, rows = 8192, 130, 2 ** 18 + 77
+    if torch.cuda.mem_get_info()[0] < 90e9:
+        pytest.skip("needs 90 GB")
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.empty(rows, d, device=cuda)
+    x.normal_(generator=g)
+    wg, wu, wd = (torch.randn(*s, generator=g, device=cuda) * 0.02 for s in ((d, f), (d, f), (f, d)))
+    last = 205                                   # 256 * 1024 + 77 ends 77 rows into a block
+    y, saved = mf.gated_ffn(x, wg, wu, wd, save=True)
+    close(y[-last:], want(x[-last:], wg, wu, wd, x[-last:], "silu")["y"], "y")
+    del y
+    grad = torch.zeros(rows, d, device=cuda)
+    grad[-77:].normal_(generator=g)              # the rest adds nothing to the weights' gradients
+    dx, *dw = mf.gated_ffn_backward(grad, x, wg, wu, wd, saved=saved)
+    pairs = want(x[-77:], wg, wu, wd, grad[-77:], "silu")
+    close(dx[-77:], pairs["dx"], "dx")
+    for got, name in zip(dw, ("dwg", "dwu", "dwd")):
+        close(got, pairs[name], name)
+    assert not dx[:-77].any()
+    assert mf.device_status() == 0
