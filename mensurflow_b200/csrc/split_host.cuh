@@ -214,8 +214,8 @@ int x_slots(XWorkspace& ws, int kind, int cluster, int* slots) {
 }
 
 // Time of a launch in SM cycles: whole waves of tiles, and the part of the epilogue that no product
-// hides. A chunk of 128 takes 24 MMAs: 3072 cycles for a pair's 256 x 256, which it reaches (its
-// 128 KB per CTA come at 42 bytes a cycle). One CTA's 128 x 128 would take 1536, but 128 KB in that
+// hides. A chunk of 128 takes 24 MMAs, of 128 cycles for a pair's 256 x 256, which it reaches (its
+// 128 KB per CTA come at 42 bytes a cycle). One CTA's 128 x 128 would take 24 x 64, but 128 KB in that
 // time is more than an SM gets from L2: 2500 measured (4 to 50 chunks), and 4200 for 128 x 256.
 // Sharing a contraction costs 9000 cycles (128 x 128) or 17000 per wave (1024 x 1024 over a depth
 // of 1024: 15.6 us by clusters of 3 single CTAs, 24.5 us by clusters of 4 pairs).
@@ -299,7 +299,7 @@ int x_product(XWorkspace& ws, mfk::XArgs& g, int64_t k0, int64_t k1, int64_t bat
         rc = s == 1 ? x_slots<2, 2, EPI, false>(ws, EPI * 12 + s - 1, 2, &slots)
                     : x_slots<2, 2, EPI, true>(ws, EPI * 12 + s - 1, 2 * s, &slots);
         if (rc != MFK_OK) return rc;
-        consider(2, s, tiles2, 3072.0, kEpi2, 17000.0);
+        consider(2, s, tiles2, 24 * 128.0, kEpi2, 17000.0);
     }
     for (int s = 1; s <= 8 && s <= g.kc; ++s) {
         rc = s == 1 ? x_slots<1, kNb1, EPI, false>(ws, EPI * 12 + 3 + s, 1, &slots)

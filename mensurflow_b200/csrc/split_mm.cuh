@@ -15,10 +15,10 @@
 //
 // Accumulation. tcgen05 rounds its fp32 accumulator toward zero on every instruction: each one
 // loses about 3.4e-8 of the running sum, always towards zero (measured: 3.8e-6 relative to the
-// result after 192 instructions, 1.2e-5 after 3072 spread over stream-K parts). So a tensor-memory
-// accumulator only ever holds one 128-deep chunk (24 instructions, the small lo products of a stage
-// first), and the epilogue warps add the chunks, scaled by the two blocks' 1/s, in fp32 registers
-// with round to nearest.
+// result after 192 instructions, 1.2e-5 after sixteen times as many spread over stream-K parts). So
+// a tensor-memory accumulator only ever holds one 128-deep chunk (24 instructions, the small lo
+// products of a stage first), and the epilogue warps add the chunks, scaled by the two blocks' 1/s,
+// in fp32 registers with round to nearest.
 //
 // Layout. A block is 64 KB: hi then lo, each as 16 columns-of-eight ("lines"), a line holding
 // 128 rows x 8 halves (16 bytes a row, 2 KB). 8 rows x 16 bytes are one core matrix of the
