@@ -18,6 +18,18 @@ int launch_embedding(const float* table, int64_t rows, int64_t d, int64_t ld, co
                      cudaStream_t stream) {
     const int vec = d % 4 == 0 && ld % 4 == 0 && ld_out % 4 == 0 && aligned16(table) &&
                     aligned16(out);
+    if (d <= 128) {
+        int lanes = 1;
+        while (lanes < 32 && lanes * (vec ? 4 : 1) < d) lanes *= 2;
+        const int64_t per_block = 8 * 4 * (32 / lanes);
+        auto kernel =
+            vec ? mfk::embedding_narrow_kernel<ID, 4> : mfk::embedding_narrow_kernel<ID, 1>;
+        kernel<<<static_cast<unsigned>((n + per_block - 1) / per_block), 256, 0, stream>>>(
+            table, rows, static_cast<int>(d), ld, ids, n, scale, out, ld_out, lanes);
+        g_launches.fetch_add(1);
+        MFK_CUDA(cudaGetLastError());
+        return MFK_OK;
+    }
     const int64_t warps = n * ((d + 511) / 512);
     const int64_t blocks = std::min<int64_t>((warps + 7) / 8, int64_t(info->sm_count) * 64);
     mfk::embedding_kernel<ID><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(

@@ -177,3 +177,29 @@ def test_offsets_past_32_bits(cuda):
     out[ids] = 0.0
     assert not out.any()
     assert mf.device_status() == 0
+
+
+@pytest.mark.parametrize("d", [1, 3, 4, 16, 17, 31, 33, 64, 100, 128, 129, 132, 256, 260, 511, 512, 515])
+@pytest.mark.parametrize("n,rows", [(1, 4), (130, 40), (6000, 3), (40000, 30000)])
+def test_narrow_rows(cuda, n, rows, d):
+    """Rows that fill part of a warp or block: several tokens or windows beside each other, and one
+    run longer than a window's block."""
+    g = torch.Generator(device="cuda").manual_seed(n + rows + d)
+    ids = (torch.rand(n, generator=g, device=cuda) ** 4 * rows).long().clamp_(max=rows - 1)
+    ids[n // 3: n // 2] = rows // 2
+    table = torch.randn(rows, d, generator=g, device=cuda)
+    grad = torch.randn(n, d, generator=g, device=cuda)
+    assert torch.equal(mf.embedding(table, ids, 0.3), table[ids] * 0.3)
+    got = mf.embedding_grad(grad, ids, rows, 0.3)
+    close(got, grad, ids, rows, 0.3)
+    assert torch.equal(got, mf.embedding_grad(grad, ids, rows, 0.3))
+    base = torch.full((rows, d + 3), -7.0, device=cuda)      # unaligned rows
+    base[:, 1:d + 1] = table
+    assert torch.equal(mf.embedding(base[:, 1:d + 1], ids, 0.3), table[ids] * 0.3)
+    wide = torch.cat([grad, grad], -1)
+    close(mf.embedding_grad(wide[:, d:], ids, rows, 0.3), grad, ids, rows, 0.3)
+    ids[0] = rows
+    y = mf.embedding(table, ids)
+    assert not y[0].any() and torch.equal(y[1:], table[ids[1:]])
+    assert mf.device_status() == 0x20
+    assert mf.device_status() == 0
