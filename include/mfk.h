@@ -366,7 +366,7 @@ int mfk_copy_peer(void* dst, int32_t dst_device, const void* src, int32_t src_de
  * strides; of each output's strides one must be 1. The gradients are written, not added to, and
  * must not overlap the inputs or each other. rows = 0 gives zero weight gradients. A row whose
  * grad is all zero (padding) adds nothing to the weight gradients, whatever finite or non-finite
- * values x has there.
+ * values x has there, and with finite weights its dx is zero.
  *
  * Both take their workspace from the stream-ordered allocator. */
 typedef struct mfk_gated_ffn_desc {

@@ -185,8 +185,8 @@ def gated_ffn_backward(grad: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor
     arguments; dx has x's shape and the weights' gradients have the weights' own layouts.
     ``saved`` from the forward call with the same x and weights; without it the two projections
     are computed again. What is not needed is None. A row whose gradient is all zero (padding) adds
-    nothing to the weights' gradients, whatever x holds there. Arithmetic as in ``gated_ffn``, with
-    one scale per 128 x 128 block."""
+    nothing to the weights' gradients, whatever x holds there, and its dx is zero. Arithmetic as in
+    ``gated_ffn``, with one scale per 128 x 128 block."""
     op = "gated_ffn_backward"
     desc, keep = _gated_args(op, x, w_gate, w_up, w_down, activation, transpose_w)
     _require(grad, op, "grad")

@@ -1214,7 +1214,8 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
             // (the maxima over the row's 64 columns): a scale a few powers of two above the
             // tightest one moves the range of a floating format, not its precision, and saves a
             // pass. A row without a gradient has no part in any sum over rows, whatever is in it:
-            // its h is left out, and its size does not count.
+            // its dgate, dup and h are zeros (as computed they would be 0 times gate and up, which
+            // need not be finite there), and its size does not count.
             uint32_t* slot = red + parity * 8;
             const int grow = i * kXBlk + row;
             const bool live = grow < g.m && g.live[grow] != 0;
@@ -1290,7 +1291,11 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
                                 const float2 h = mul2(ac, u);
                                 dg[x] = p.x, dg[x + 1] = p.y;
                                 du[x] = q.x, du[x + 1] = q.y;
-                                hh[x] = live ? h.x : 0.0f, hh[x + 1] = live ? h.y : 0.0f;
+                                hh[x] = h.x, hh[x + 1] = h.y;
+                            }
+                            if (!live) {
+#pragma unroll
+                                for (int x = 0; x < 8; ++x) dg[x] = du[x] = hh[x] = 0.0f;
                             }
                             store_split8(g.o[0].data + off, half * 8 + ch0 + ch, row, dg, s0);
                             store_split8(g.o[1].data + off, half * 8 + ch0 + ch, row, du, s1);

@@ -421,3 +421,23 @@ def test_offsets_past_32_bits(cuda):
         close(got, pairs[name], name)
     assert not dx[:-77].any()
     assert mf.device_status() == 0
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu", None])
+@pytest.mark.parametrize("filler", [float("nan"), float("inf"), -float("inf"), 3e38])
+def test_rows_without_a_gradient_may_hold_anything(cuda, act, filler):
+    """Rows whose gradient is zero add nothing and get a zero dx where x is not finite, or finite
+    and the projections overflow: in whole rows and in single entries."""
+    x, wg, wu, wd, dy = inputs(cuda, 210, 130, 190)
+    dy[150:] = 0
+    ref = want(x[:150], wg, wu, wd, dy[:150], act)
+    x[150:200] = filler
+    x[201:, 5] = filler
+    for keep in (True, False):
+        saved = mf.gated_ffn(x, wg, wu, wd, act, save=True)[1] if keep else None
+        dx, *dw = mf.gated_ffn_backward(dy, x, wg, wu, wd, act, saved=saved)
+        assert (dx[150:] == 0).all()
+        close(dx[:150], ref["dx"], "dx")
+        for got, name in zip(dw, ("dwg", "dwu", "dwd")):
+            close(got, ref[name], name)
+    assert mf.device_status() == 0
