@@ -351,7 +351,8 @@ int mfk_copy_peer(void* dst, int32_t dst_device, const void* src, int32_t src_de
  * of h have a scale each per 128 columns, so no row of y depends on another; the weights, and in
  * the backward pass every matrix, have one per 128 x 128 block. Under one scale an entry keeps 22
  * bits or more while it is within 2^-17 of the largest, and an absolute error of 2^-39 of that one
- * below. A non-finite operand entry makes the results that depend on it non-finite (an infinity may
+ * below; dgate, dup and h of the backward pass, whose scales may be three powers of two larger,
+ * within 2^-14, and 2^-36 below. A non-finite operand entry makes the results that depend on it non-finite (an infinity may
  * come out as NaN). Up to 16 rows without `saved` are plain fp32 sums.
  *
  * mfk_gated_ffn_f32: y has row stride ldy >= d. saved (optional, 16-byte aligned,

@@ -186,7 +186,9 @@ def gated_ffn_backward(grad: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor
     ``saved`` from the forward call with the same x and weights; without it the two projections
     are computed again. What is not needed is None. A row whose gradient is all zero (padding) adds
     nothing to the weights' gradients, whatever x holds there, and its dx is zero. Arithmetic as in
-    ``gated_ffn``, with one scale per 128 x 128 block."""
+    ``gated_ffn``, with one scale per 128 x 128 block: an entry of grad more than 2^17 below the
+    largest of its block keeps an absolute error of 2^-39 of that one, an entry of the hidden values
+    and their gradients more than 2^14 below one of 2^-36."""
     op = "gated_ffn_backward"
     desc, keep = _gated_args(op, x, w_gate, w_up, w_down, activation, transpose_w)
     _require(grad, op, "grad")

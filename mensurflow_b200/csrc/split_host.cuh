@@ -5,7 +5,7 @@
 
 namespace {
 
-constexpr int kXKinds = 60;  // kernel instantiations (and cluster sizes) with per-device set-up
+constexpr int kXKinds = 72;  // kernel instantiations (and cluster sizes) with per-device set-up
 
 struct XDevice {
     bool ready[kXKinds] = {};
@@ -510,11 +510,15 @@ int run_gated_ffn_backward(const mfk_gated_ffn_desc* d, const mfk_gated_ffn_grad
     const XMat h = x_mat(ws, d->rows, d->f);
     const int64_t saved_floats = gated_saved_floats(d->rows, d->f);
     const size_t again = saved == nullptr ? static_cast<size_t>(saved_floats) : 0;
-    rc = x_allocate(ws, again + static_cast<size_t>(d->rows));
+    const size_t live_words = (static_cast<size_t>(d->rows) + 3) / 4 * 4;
+    const int64_t top_words = h.blocks() * 4;
+    rc = x_allocate(ws, again + live_words + static_cast<size_t>(top_words));
     if (rc != MFK_OK) return rc;
     int* live = reinterpret_cast<int*>(ws.extra + again);
+    uint32_t* tops = reinterpret_cast<uint32_t*>(live + live_words);
     mfk::live_rows_kernel<<<static_cast<unsigned>((d->rows + 7) / 8), 256, 0, stream>>>(
-        o->grad, o->grad_rs, o->grad_cs, static_cast<int>(d->rows), static_cast<int>(d->d), live);
+        o->grad, o->grad_rs, o->grad_cs, static_cast<int>(d->rows), static_cast<int>(d->d), live,
+        tops, top_words);
     g_launches.fetch_add(1);
     MFK_CUDA(cudaGetLastError());
     list.s[0].live = live;
@@ -542,10 +546,17 @@ int run_gated_ffn_backward(const mfk_gated_ffn_desc* d, const mfk_gated_ffn_grad
         g.up = p + blocks * 128 * 128;
         g.gmax = p + blocks * 2 * 128 * 128;
         g.live = live;
+        g.tops = tops;
         g.o[0] = x_out(ws, dg);
         g.o[1] = x_out(ws, du);
         g.o[2] = x_out(ws, h);
         rc = x_product<mfk::kXGatedBwd>(ws, g, d->d, 0, 1);
+        if (rc != MFK_OK) return rc;
+        // the blocks that it stored under loose scales, by tiles of one CTA
+        int slots = 0;
+        rc = x_slots<1, 1, mfk::kXGatedAgain, false>(ws, mfk::kXGatedAgain * 12 + 4, 1, &slots);
+        if (rc != MFK_OK) return rc;
+        rc = x_launch<1, 1, mfk::kXGatedAgain, false>(ws, g, slots, 1, g.mb, g.nb, blocks, 1);
         if (rc != MFK_OK) return rc;
     }
     if (need_x) {  // dx = dgate w_gate^T + dup w_up^T: one product over 2 f

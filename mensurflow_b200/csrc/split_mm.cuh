@@ -46,12 +46,20 @@ constexpr int kXEpiThreads = 256;
 constexpr int kXBoxFloats = 32 * 32;
 
 // kXWeights: fp32 results of three products in one launch, two of one shape (a batch) and a third
-// with sizes and operands of its own over the same depth.
-enum XEpi : int { kXF32 = 0, kXSplit = 1, kXGated = 2, kXGatedBwd = 3, kXWeights = 4 };
+// with sizes and operands of its own over the same depth. kXGatedAgain: kXGatedBwd for the blocks
+// that it stored under loose scales.
+enum XEpi : int {
+    kXF32 = 0, kXSplit = 1, kXGated = 2, kXGatedBwd = 3, kXWeights = 4, kXGatedAgain = 5
+};
 
 template <int EPI>
 __host__ __device__ constexpr bool x_fp32() {
     return EPI == kXF32 || EPI == kXWeights;
+}
+
+template <int EPI>
+__host__ __device__ constexpr bool x_backward() {
+    return EPI == kXGatedBwd || EPI == kXGatedAgain;
 }
 
 // A split matrix as an operand: block (mn, k) of matrix z.
@@ -94,6 +102,7 @@ struct XArgs {
     float* up;
     float* gmax;           // largest |gate| and |up| of 64 columns: per block [2][2 halves][128]
     const int* live;       // backward: 0 for the rows whose gradient is all zero
+    uint32_t* tops;        // backward, per block: fp16 bits of the largest |hi| of dgate, dup, h; 0
     int act;
     int store_h;
 };
@@ -293,14 +302,21 @@ __device__ __forceinline__ void split_pair(float x0, float x1, float s, uint32_t
     lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
-// Eight consecutive columns (16-byte line `chunk`) of one row of a block.
+// Eight consecutive columns (16-byte line `chunk`) of one row of a block; `top` gathers the largest
+// |hi| of even and odd columns.
 __device__ __forceinline__ void store_split8(uint8_t* block, int chunk, int row, const float* v,
-                                             float s) {
+                                             float s, __half2* top = nullptr) {
     uint4 h, l;
     split_pair(v[0], v[1], s, h.x, l.x);
     split_pair(v[2], v[3], s, h.y, l.y);
     split_pair(v[4], v[5], s, h.z, l.z);
     split_pair(v[6], v[7], s, h.w, l.w);
+    if (top != nullptr) {
+        const uint32_t hs[4] = {h.x, h.y, h.z, h.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *top = __hmax2(*top, __habs2(*reinterpret_cast<const __half2*>(&hs[i])));
+    }
     uint8_t* p = block + chunk * kXLineBytes + row * 16;
     *reinterpret_cast<uint4*>(p) = h;
     *reinterpret_cast<uint4*>(p + kXBlockBytes / 2) = l;
@@ -474,13 +490,15 @@ __global__ void __launch_bounds__(256) split_blocks_kernel(const __grid_constant
 }
 
 // live[r] = whether row r of the rows x cols matrix has an entry other than zero: a warp per row,
-// which stops at the first 32 columns that have one.
+// which stops at the first 32 columns that have one. Clears `words` words at `clear`.
 __global__ void __launch_bounds__(256)
     live_rows_kernel(const float* __restrict__ p, long long rs, long long cs, int rows, int cols,
-                     int* __restrict__ live) {
+                     int* __restrict__ live, uint32_t* __restrict__ clear, long long words) {
     grid_dependents_go();
+    const long long t = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+    for (long long i = t; i < words; i += static_cast<long long>(gridDim.x) * 256) clear[i] = 0u;
     const int lane = threadIdx.x & 31;
-    const int r = static_cast<int>((static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) >> 5);
+    const int r = static_cast<int>(t >> 5);
     if (r >= rows) return;
     bool any = false;
     for (int c = 0; c < cols && !any; c += 32) {
@@ -610,6 +628,15 @@ __device__ __forceinline__ void with_act(int act, F&& f) {
 // The largest |act'| over all inputs (GELU's is 1.1290): bounds the gate's gradient.
 constexpr float kXMaxSlope = 1.13f;
 
+// fp16 bits of 2^11: a block whose scale brought a bound into [2^14, 2^15) and whose largest |hi| is
+// below, or infinite, has a scale that is more than three powers of two off, or unknown.
+constexpr uint32_t kXTight = 0x6800u;
+constexpr float kXMostScale = 8.507059173e37f;  // 2^126, the largest that split_scale gives
+
+__device__ __forceinline__ bool x_loose(uint32_t top) {
+    return top < kXTight || top >= 0x7c00u;
+}
+
 // ---- the product -----------------------------------------------------------------------------
 
 template <int CG, int NB>
@@ -661,6 +688,18 @@ __device__ __forceinline__ XUnit x_unit(const XArgs& g, int u) {
     return w;
 }
 
+// Whether a launch has nothing to do in this tile.
+template <int EPI>
+__device__ __forceinline__ bool x_skips(const XArgs& g, const XUnit& w) {
+    if constexpr (EPI == kXGatedAgain) {
+        const uint4 t = __ldcg(reinterpret_cast<const uint4*>(g.tops) +
+                               (static_cast<long long>(w.tm) * g.nb + w.tn));
+        return !x_loose(t.x) && !x_loose(t.y) && !x_loose(t.z);
+    } else {
+        return false;
+    }
+}
+
 // Whether a tile whose first block along the operand's mn is `mn0` reads chunk k along the
 // blocks' stored rows (MN-major). A symmetric matrix stores only its lower blocks: a chunk right
 // of the tile's first block comes from (k, mn), transposed. All blocks of one MMA agree: for
@@ -703,6 +742,7 @@ __device__ __forceinline__ void x_producer(const XArgs& g, const CUtensorMap* mk
     uint32_t phase = 0;
     for (int u = first; u < g.units; u += step) {
         const XUnit w = x_unit<EPI>(g, u);
+        if (x_skips<EPI>(g, w)) continue;
         const int nb = x_third<EPI>(w.z) ? g.third.nb : g.nb;
         const int i = min(w.tm * CG + static_cast<int>(rank),
                           (x_third<EPI>(w.z) ? g.third.mb : g.mb) - 1);
@@ -761,6 +801,7 @@ __device__ __forceinline__ void x_mma(const XArgs& g, uint32_t tmem, uint8_t* st
     const uint32_t stage0 = smem_u32(stages);
     for (int u = first; u < g.units; u += step) {
         const XUnit w = x_unit<EPI>(g, u);
+        if (x_skips<EPI>(g, w)) continue;
         const int i = w.tm * CG, j = EPI == kXGated ? w.tn : w.tn * NB;
         for (int c = w.c0; c < w.c1; ++c) {
             const int seg = x_third<EPI>(w.z) || (EPI == kXF32 && c >= g.kc0) ? 1 : 0;
@@ -830,9 +871,13 @@ __device__ __forceinline__ void x_mma(const XArgs& g, uint32_t tmem, uint8_t* st
 // The largest of a value over the epilogue's threads, in a shared slot. Three sets of slots take
 // turns: before a tile's barrier the next tile's set is cleared, which was last read before the
 // barrier of the tile before.
-__device__ __forceinline__ void x_max_into(uint32_t* red, float amax) {
-    const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(amax));
+__device__ __forceinline__ void x_max_into(uint32_t* red, uint32_t bits) {
+    const uint32_t m = __reduce_max_sync(0xffffffffu, bits);
     if ((threadIdx.x & 31) == 0) atomicMax(red, m);
+}
+
+__device__ __forceinline__ void x_max_into(uint32_t* red, float amax) {
+    x_max_into(red, __float_as_uint(amax));
 }
 
 // Thread (quarter q, half h, lane) owns row 32 q + lane of the CTA's 128 and, of every 128-column
@@ -859,6 +904,7 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
     bool alive = true;  // a wait that gave up: finish without waiting, so every barrier is met
     for (int u = first; u < g.units; u += step) {
         const XUnit w = x_unit<EPI>(g, u);
+        if (x_skips<EPI>(g, w)) continue;
         const int i = w.tm * CG + static_cast<int>(rank);
         const bool third = x_third<EPI>(w.z);
         const int mb = third ? g.third.mb : g.mb, nb = third ? g.third.nb : g.nb;
@@ -870,15 +916,15 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
         // warp's box, each lane copying what it reads itself: the backward's gate and up in two
         // slots, a split C in four. The first turns while the product is still computed (C read
         // when it was needed made the tail of a 1024 x 4096 product 6 us instead of 4).
-        constexpr int kSlots = EPI == kXGatedBwd ? 2 : 4;
+        constexpr int kSlots = x_backward<EPI>() ? 2 : 4;
         const bool reads =
-            EPI == kXGatedBwd || ((EPI == kXF32 || EPI == kXSplit) && g.beta != 0.0f);
+            x_backward<EPI>() || ((EPI == kXF32 || EPI == kXSplit) && g.beta != 0.0f);
         const int turns = reads && i < g.mb ? min(NB, g.nb - w.tn * NB) * ng : 0;
         auto fetch = [&](int turn) {
             if (turn < turns) {
                 const int b = SPL ? turn / ng : turn >> 3, ch = turn - b * ng;
                 const uint32_t dst = smem_u32(box) + (turn % kSlots) * (4096 / kSlots) + lane * 16;
-                if constexpr (EPI == kXGatedBwd) {
+                if constexpr (x_backward<EPI>()) {
                     const long long at =
                         ((static_cast<long long>(i * g.o[0].ldb + w.tn * NB + b) * 2 + half) * 64 +
                          (ch0 + ch) * 8) * kXBlk + row * 4;
@@ -901,7 +947,7 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
 #pragma unroll
             for (int t = 0; t < kSlots; ++t) fetch(t);
         }
-        if constexpr (EPI == kXGatedBwd) {
+        if constexpr (x_backward<EPI>()) {
             for (int b = 0; b < NB; ++b) {
                 const int jb = w.tn * NB + b;
                 if (i < g.mb && jb < g.nb && w.s == 0) {
@@ -1207,68 +1253,81 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
             }
         }
 
-        if constexpr (EPI == kXGatedBwd) {
-            // acc: the gradient of h. The three outputs' scales come from bounds, the largest over
-            // a block's rows of
+        if constexpr (x_backward<EPI>()) {
+            // acc: the gradient of h. The three outputs are stored under scales from bounds, the
+            // largest over a block's rows of
             // |dgate| <= 1.13 max|dh| max|up|, |dup| <= max|dh| max|gate|, |h| <= max|gate| max|up|
-            // (the maxima over the row's 64 columns): a scale a few powers of two above the
-            // tightest one moves the range of a floating format, not its precision, and saves a
-            // pass. A row without a gradient has no part in any sum over rows, whatever is in it:
-            // its dgate, dup and h are zeros (as computed they would be 0 times gate and up, which
-            // need not be finite there), and its size does not count.
+            // (the maxima over the row's 64 columns), and the largest |hi| is kept. On ordinary rows
+            // a bound is up to three powers of two too large, which leaves an entry its 22 bits down
+            // to 2^-14 of the largest. Where gates are saturated, act and act' are tiny and it can
+            // be any number too large (2^25 for SiLU at -20): such blocks are computed once more by
+            // the next launch (kXGatedAgain), which looks for their largest values first. (8192 x
+            // 4096 x 11008: 1800 us with bounds alone, 1835 so, and 5 for a next launch that finds
+            // nothing to do; 2070 in one launch that stores loose blocks twice, because a pair's 128
+            // sums a thread stay alive for that.)
+            // A row without a gradient has no part in any sum over rows, whatever is in it: its
+            // dgate, dup and h are zeros (as computed they would be 0 times gate and up, which need
+            // not be finite there), and its size does not count.
             uint32_t* slot = red + parity * 8;
             const int grow = i * kXBlk + row;
             const bool live = grow < g.m && g.live[grow] != 0;
+            auto gathered = [&]() {
+                parity = parity == 2 ? 0 : parity + 1;
+                if (et < 8) red[parity * 8 + et] = 0u;
+                epi_bar();
+            };
+            uint32_t top_of[NB * 3] = {};
+            if constexpr (EPI == kXGatedBwd) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const int jb = w.tn * NB + b;
-                if (row_block && jb < g.nb) {
-                    const float* from = g.gmax +
-                                        static_cast<long long>(i * g.o[0].ldb + jb) * 4 * kXBlk +
-                                        half * kXBlk + row;
-                    const float gm = live ? from[0] : 0.0f, um = live ? from[2 * kXBlk] : 0.0f;
-                    const float dm = largest<64>(acc + b * 64);
-                    const float top = 3.402823466e38f;
-                    x_max_into(slot + b * 3, fminf(dm * um * kXMaxSlope, top));
-                    x_max_into(slot + b * 3 + 1, fminf(dm * gm, top));
-                    x_max_into(slot + b * 3 + 2, fminf(gm * um, top));
-                }
-            }
-            parity = parity == 2 ? 0 : parity + 1;
-            if (et < 8) red[parity * 8 + et] = 0u;
-            epi_bar();
-            uint32_t top_of[NB * 3];
-#pragma unroll
-            for (int e = 0; e < NB * 3; ++e) top_of[e] = slot[e];
-            if constexpr (SPL) {
-                cluster_sync();
-                for (int r = 0; r < g.splits; ++r) {
-                    const uint32_t at = mapa_shared(slot, r * CG + rank);
-#pragma unroll
-                    for (int e = 0; e < NB * 3; ++e)
-                        top_of[e] = max(top_of[e], ld_cluster_u32(at + e * 4));
-                }
-            }
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const int jb = w.tn * NB + b;
-                if (row_block && jb < g.nb) {
-                    const int blk = i * g.o[0].ldb + jb;
-                    float s0, s1, s2, i0, i1, i2;
-                    split_scale(__uint_as_float(top_of[b * 3]), s0, i0);
-                    split_scale(__uint_as_float(top_of[b * 3 + 1]), s1, i1);
-                    split_scale(__uint_as_float(top_of[b * 3 + 2]), s2, i2);
-                    if (et == 0 && w.s == 0) {
-                        g.o[0].inv[blk] = i0;
-                        g.o[1].inv[blk] = i1;
-                        g.o[2].inv[blk] = i2;
+                for (int b = 0; b < NB; ++b) {
+                    const int jb = w.tn * NB + b;
+                    if (row_block && jb < g.nb) {
+                        const float* from =
+                            g.gmax + static_cast<long long>(i * g.o[0].ldb + jb) * 4 * kXBlk +
+                            half * kXBlk + row;
+                        const float gm = live ? from[0] : 0.0f, um = live ? from[2 * kXBlk] : 0.0f;
+                        const float dm = largest<64>(acc + b * 64);
+                        const float top = 3.402823466e38f;
+                        x_max_into(slot + b * 3, fminf(dm * um * kXMaxSlope, top));
+                        x_max_into(slot + b * 3 + 1, fminf(dm * gm, top));
+                        x_max_into(slot + b * 3 + 2, fminf(gm * um, top));
                     }
+                }
+                gathered();
+#pragma unroll
+                for (int e = 0; e < NB * 3; ++e) top_of[e] = slot[e];
+                if constexpr (SPL) {
+                    cluster_sync();
+                    for (int r = 0; r < g.splits; ++r) {
+                        const uint32_t at = mapa_shared(slot, r * CG + rank);
+#pragma unroll
+                        for (int e = 0; e < NB * 3; ++e)
+                            top_of[e] = max(top_of[e], ld_cluster_u32(at + e * 4));
+                    }
+                }
+            }
+            // kXGatedAgain takes the maxima in a pass of its own
+#pragma unroll 1
+            for (int pass = EPI == kXGatedAgain ? 0 : 1; pass < 2; ++pass) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    const int jb = w.tn * NB + b;
+                    if (!row_block || jb >= g.nb) continue;
+                    const int blk = i * g.o[0].ldb + jb;
                     const long long off = static_cast<long long>(blk) * kXBlockBytes;
+                    float sc[3], most[3] = {};
+                    __half2 hi[3] = {};
+#pragma unroll
+                    for (int e = 0; e < 3; ++e) {
+                        float inv;
+                        split_scale(__uint_as_float(max(top_of[b * 3 + e], 1u)), sc[e], inv);
+                        if (pass == 1 && et == 0 && w.s == 0) g.o[e].inv[blk] = inv;
+                    }
                     with_act(g.act, [&](auto kind) {
 #pragma unroll
                         for (int ch = 0; ch < 8; ++ch) {
                             if (SPL && ch >= ng) break;
-                            float dg[8], du[8], hh[8];
+                            float out3[3][8];   // dgate, dup, h
                             const int turn = b * ng + ch;
                             const uint32_t src =
                                 smem_u32(box) + (turn % kSlots) * (4096 / kSlots) + lane * 16;
@@ -1289,23 +1348,52 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
                                                                   sl);
                                 const float2 p = mul2(mul2(dh, u), sl), q = mul2(dh, ac);
                                 const float2 h = mul2(ac, u);
-                                dg[x] = p.x, dg[x + 1] = p.y;
-                                du[x] = q.x, du[x + 1] = q.y;
-                                hh[x] = h.x, hh[x + 1] = h.y;
+                                out3[0][x] = p.x, out3[0][x + 1] = p.y;
+                                out3[1][x] = q.x, out3[1][x + 1] = q.y;
+                                out3[2][x] = h.x, out3[2][x + 1] = h.y;
                             }
                             if (!live) {
 #pragma unroll
-                                for (int x = 0; x < 8; ++x) dg[x] = du[x] = hh[x] = 0.0f;
+                                for (int x = 0; x < 8; ++x)
+                                    out3[0][x] = out3[1][x] = out3[2][x] = 0.0f;
                             }
-                            store_split8(g.o[0].data + off, half * 8 + ch0 + ch, row, dg, s0);
-                            store_split8(g.o[1].data + off, half * 8 + ch0 + ch, row, du, s1);
-                            store_split8(g.o[2].data + off, half * 8 + ch0 + ch, row, hh, s2);
+#pragma unroll
+                            for (int e = 0; e < 3; ++e) {
+                                if (pass == 0)
+                                    most[e] = fmaxf(most[e], largest<8>(out3[e]));
+                                else
+                                    store_split8(g.o[e].data + off, half * 8 + ch0 + ch, row,
+                                                 out3[e], sc[e],
+                                                 EPI == kXGatedBwd ? &hi[e] : nullptr);
+                            }
                         }
                     });
+#pragma unroll
+                    for (int e = 0; e < 3; ++e) {
+                        if (pass == 0) {
+                            x_max_into(slot + e, most[e]);
+                        } else if constexpr (EPI == kXGatedBwd) {
+                            const __half t = __hmax(__low2half(hi[e]), __high2half(hi[e]));
+                            x_max_into(g.tops + static_cast<long long>(blk) * 4 + e,
+                                       sc[e] == kXMostScale
+                                           ? kXTight  // zeros, or nothing better
+                                           : static_cast<uint32_t>(__half_as_ushort(t)));
+                        }
+                    }
+                }
+                if constexpr (EPI == kXGatedAgain) {
+                    if (pass == 0) {
+                        gathered();
+#pragma unroll
+                        for (int e = 0; e < NB * 3; ++e) top_of[e] = slot[e];
+                        cp_async_wait<0>();
+#pragma unroll
+                        for (int t = 0; t < kSlots; ++t) fetch(t);
+                    }
                 }
             }
         }
-        if constexpr (EPI == kXGatedBwd) cp_async_wait<0>();
+        if constexpr (x_backward<EPI>()) cp_async_wait<0>();
         if constexpr (SPL) cluster_sync();  // nobody leaves while its sums or maxima are read
     }
 }
@@ -1368,7 +1456,16 @@ __global__ void __launch_bounds__(kXThreads, 1)
     const uint32_t tmem = *tmem_holder;
     grid_wait();  // before anything of the launch before is read or overwritten
 
-    if (warp == 0) {
+    bool work = true;
+    if constexpr (EPI == kXGatedAgain) {  // most often none of the tiles has to be done again
+        bool any = false;
+        for (int u = first + static_cast<int>(threadIdx.x) * step; u < g.units;
+             u += kXThreads * step)
+            any = any || !x_skips<EPI>(g, x_unit<EPI>(g, u));
+        work = __syncthreads_or(any) != 0;
+    }
+    if (!work) {
+    } else if (warp == 0) {
         if (lane == 0)
             x_producer<CG, NB, EPI>(g, &mk, &mm, stages, full, empty, rank, leader, first, step);
         __syncwarp();

@@ -441,3 +441,123 @@ def test_rows_without_a_gradient_may_hold_anything(cuda, act, filler):
         for got, name in zip(dw, ("dwg", "dwu", "dwd")):
             close(got, ref[name], name)
     assert mf.device_status() == 0
+
+
+def exact_projections(cuda, rows, d, f, center, seed):
+    """Inputs whose gate, up and dh are exact in fp32: gate = x[:, 0] w_gate[0] with w_gate[0]
+    within 1/4 of `center`, up = x[:, 1] w_up[1], grad and w_down in few bits. The other columns of
+    x are random and meet zeros in the weights."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    whole = lambda low, high, *s: torch.randint(low, high, s, generator=g, device=cuda).float()  # noqa: E731
+    x = torch.randn(rows, d, generator=g, device=cuda)
+    x[:, 0], x[:, 1] = 1.0, whole(1, 9, rows) / 8
+    wg, wu = torch.zeros(d, f, device=cuda), torch.zeros(d, f, device=cuda)
+    wg[0] = center + whole(-16, 17, f) / 64
+    wu[1] = whole(-16, 17, f) / 8
+    return x, wg, wu, whole(-8, 9, f, d) / 32, whole(-8, 9, rows, d) / 8
+
+
+def rounded_act(g, kind):
+    """Relative errors of act(g) and act'(g) in the kernels, from their expressions. The
+    exponential's argument z carries 2.5 roundings (6.5 for tanh-GELU's cube), |z| 2^-24 each; ex2
+    and rcp are off by 2^-22 and 2^-23, the few products by 2^-24; the derivative's factor beside the
+    exponential, one sum without cancellation for gates this far out, adds as much again."""
+    if kind == "silu":
+        z = g.abs()
+    elif kind == "gelu":
+        z = g * g / 2
+    elif kind == "gelu_tanh":
+        z = 2.6 * 2 * np.sqrt(2 / np.pi) * (g + 0.044715 * g ** 3).abs()
+    else:
+        return torch.zeros_like(g), torch.zeros_like(g)
+    a = z * 2.5 * 2.0 ** -24 + 2.0 ** -20
+    return a, 1.2 * a + 2.0 ** -21
+
+
+def check_backward_scales(got, x, wg, wu, wd, dy, kind, edh=0.0, what=""):
+    """The gradients against 64 bits where gate and up are exact and dh is off by `edh`: the
+    activation's roundings, 2^-36 of the largest entry of dgate, dup and h for the scale that a
+    block of them shares (at most three powers of two above its largest entry), and the products'
+    own error."""
+    x, wg, wu, wd, dy = (t.double() for t in (x, wg, wu, wd, dy))
+    g, u, dh = x[:, :1] @ wg[:1], x[:, 1:2] @ wu[1:2], dy @ wd.t()
+    a, s = act64(g, kind)
+    ea, es = rounded_act(g, kind)
+    h, dg, du = a * u, dh * u * s, dh * a
+    tf, tm = tol(wd.shape[0]), tol(x.shape[0])
+    floor = lambda t: 2.0 ** -36 * t.abs().max()  # noqa: E731
+    eh = h.abs() * (ea + 2.0 ** -22) + floor(h)
+    edg = dg.abs() * (es + 2.0 ** -22) + edh * (u * s).abs() + floor(dg)
+    edu = du.abs() * (ea + 2.0 ** -22) + edh * a.abs() + floor(du)
+    ref = {
+        "dx": (dg @ wg.t() + du @ wu.t(), edg @ wg.abs().t() + edu @ wu.abs().t() +
+               2 * tf * ((dg.abs() + edg) @ wg.abs().t() + (du.abs() + edu) @ wu.abs().t())),
+        "dwg": (x.t() @ dg, x.abs().t() @ (edg + tm * (dg.abs() + edg))),
+        "dwu": (x.t() @ du, x.abs().t() @ (edu + tm * (du.abs() + edu))),
+        "dwd": (h.t() @ dy, (eh + tm * (h.abs() + eh)).t() @ dy.abs()),
+    }
+    for t, name in zip(got, ("dx", "dwg", "dwu", "dwd")):
+        close(t, ref[name], f"{what} {name}")
+
+
+@pytest.mark.parametrize("act,center", [("silu", -20.0), ("silu", -40.0), ("gelu", -6.0),
+                                        ("gelu_tanh", -5.0), ("gelu", 6.0), ("relu", -1.0)])
+@pytest.mark.parametrize("shape", [(200, 96, 160), (3, 40, 130), (2100, 70, 2600),
+                                   (520, 2000, 300), (1900, 4096, 2000), (1000, 8192, 1000)])
+def test_saturated_gates(cuda, act, center, shape):
+    """Blocks whose gates are all far out, where act and act' are tiny beside gate and up: the
+    gradients keep their bits. Tiles of one CTA and of pairs, with the contraction shared by a
+    cluster and not."""
+    x, wg, wu, wd, dy = exact_projections(cuda, *shape, center, 7)
+    for keep in (True, False):
+        saved = mf.gated_ffn(x, wg, wu, wd, act, save=True)[1] if keep else None
+        got = mf.gated_ffn_backward(dy, x, wg, wu, wd, act, saved=saved)
+        check_backward_scales(got, x, wg, wu, wd, dy, act, what=str(keep))
+    assert mf.device_status() == 0
+
+
+@pytest.mark.parametrize("act", ["silu", "relu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("shape", [(200, 96, 160), (2100, 70, 2600)])
+def test_closed_gates_beside_ordinary_rows(cuda, act, shape):
+    """Rows with a gate of -2^16 and an up projection of up to 2^16: their h, dgate and dup are
+    zero, and the other rows of the block keep their bits."""
+    x, wg, wu, wd, dy = exact_projections(cuda, *shape, 1.0, 8)
+    for row in (5, 140, shape[0] - 1):
+        x[row, 0], x[row, 1] = -2.0 ** 16, 2.0 ** 16
+    y, saved = mf.gated_ffn(x, wg, wu, wd, act, save=True)
+    for s in (saved, None):
+        got = mf.gated_ffn_backward(dy, x, wg, wu, wd, act, saved=s)
+        check_backward_scales(got, x, wg, wu, wd, dy, act)
+    assert mf.device_status() == 0
+
+
+@pytest.mark.parametrize("act,center", [("silu", -20.0), ("gelu", -6.0)])
+def test_overflow_beside_saturated_gates(cuda, act, center):
+    """A row whose up projection overflows says nothing about its block's scale: the other rows' dx
+    keep their bits."""
+    x, wg, wu, wd, dy = exact_projections(cuda, 200, 96, 160, center, 10)
+    wu[1] = wu[1].abs() + 1.5                    # times 3e38: every entry of the row overflows
+    other = x.clone()
+    other[140, 1] = 3e38
+    for keep in (True, False):
+        saved = mf.gated_ffn(other, wg, wu, wd, act, save=True)[1] if keep else None
+        dx = mf.gated_ffn_backward(dy, other, wg, wu, wd, act, saved=saved)[0]
+        assert not torch.isfinite(dx[140]).all()
+        dx[140] = 0
+        zero = dy.clone()
+        zero[140] = 0
+        check_backward_scales((dx,), x, wg, wu, wd, zero, act)
+    assert mf.device_status() == 0
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_gradients_of_very_different_size(cuda, act):
+    """Rows whose gradients lie 2^-12 to 2^-36 below their neighbours': a block of grad shares one
+    scale, so an entry is off by 2^-39 of the block's largest at most, and dx's rows by what follows
+    from that."""
+    x, wg, wu, wd, dy = exact_projections(cuda, 300, 96, 260, 0.5, 9)
+    dy *= torch.pow(2.0, -12.0 * (torch.arange(300, device=cuda) % 4))[:, None]
+    edh = 2.0 ** -39 * float(dy.abs().max()) * wd.double().abs().sum(1)[None, :]
+    got = mf.gated_ffn_backward(dy, x, wg, wu, wd, act)
+    check_backward_scales(got, x, wg, wu, wd, dy, act, edh=edh)
+    assert mf.device_status() == 0
