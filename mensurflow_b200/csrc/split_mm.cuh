@@ -102,7 +102,7 @@ struct XArgs {
     float* up;
     float* gmax;           // largest |gate| and |up| of 64 columns: per block [2][2 halves][128]
     const int* live;       // backward: 0 for the rows whose gradient is all zero
-    uint32_t* tops;        // backward, per block: fp16 bits of the largest |hi| of dgate, dup, h; 0
+    uint32_t* tops;        // backward, per block: fp16 bits of the largest |hi| of dgate, dup, h
     int act;
     int store_h;
 };
@@ -547,6 +547,15 @@ __device__ __forceinline__ float rcp(float x) {
     return y;
 }
 
+// v within [-16, 16], NaN as it is.
+__device__ __forceinline__ float clamp16(float v) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;\n\tmin.NaN.f32 %0, %0, %3;"
+        : "=&f"(y)
+        : "f"(v), "f"(-16.0f), "f"(16.0f));
+    return y;
+}
+
 // 1 / (1 + exp(-z)): 2^(-z log2 e) is off by |z| 2^-24 relative at most, which the 1 it is added
 // to hides wherever the result is not tiny.
 __device__ __forceinline__ float logistic(float z) {
@@ -564,8 +573,8 @@ __device__ __forceinline__ float2 act_slope(float v) {
         const float s = logistic(v);
         return make_float2(v * s, s * (1.0f + v * (1.0f - s)));
     } else if constexpr (ACT == kXActRelu) {
-        // NaN stays NaN
-        return v > 0.0f ? make_float2(v, 1.0f) : make_float2(v == v ? 0.0f : v, 0.0f);
+        const float rest = v == v ? 0.0f : v;  // NaN stays NaN, the derivative's too
+        return v > 0.0f ? make_float2(v, 1.0f) : make_float2(rest, rest);
     } else if constexpr (ACT == kXActGelu) {
         // The normal distribution's tail: 0.5 erfc(|v| / sqrt 2) = exp(-v^2 / 2) t q(t) with
         // t = 1 / (1 + |v| / 4) and q a polynomial of degree 9, fitted to 3.4e-8 of the value
@@ -587,7 +596,7 @@ __device__ __forceinline__ float2 act_slope(float v) {
         const float phi = v < 0.0f ? tail : 1.0f - tail;
         return make_float2(v * phi, fmaf(v * 0.39894228040143268f, e, phi));
     } else if constexpr (ACT == kXActGeluTanh) {
-        const float w = fminf(fmaxf(v, -16.0f), 16.0f);  // the logistic is 0 or 1 beyond
+        const float w = clamp16(v);  // the logistic is 0 or 1 beyond
         const float s = logistic(1.5957691216057308f * (w + 0.044715f * w * w * w));
         const float dz2 = 1.5957691216057308f * (1.0f + 0.134145f * w * w);
         return make_float2(v * s, s + w * s * (1.0f - s) * dz2);

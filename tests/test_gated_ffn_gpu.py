@@ -561,3 +561,21 @@ def test_gradients_of_very_different_size(cuda, act):
     got = mf.gated_ffn_backward(dy, x, wg, wu, wd, act)
     check_backward_scales(got, x, wg, wu, wd, dy, act, edh=edh)
     assert mf.device_status() == 0
+
+
+@pytest.mark.parametrize("rows", [1, 40, 300])
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu"])
+def test_a_gate_that_is_not_a_number(cuda, act, rows):
+    """One NaN in w_gate: what depends on that feature's gate is NaN, its gradient through the
+    activation's derivative too, and nothing else."""
+    x, wg, wu, wd, dy = inputs(cuda, rows, 130, 190)
+    wg[3, 77] = float("nan")
+    assert torch.isnan(mf.gated_ffn(x, wg, wu, wd, act)).all()
+    for keep in (True, False):
+        saved = mf.gated_ffn(x, wg, wu, wd, act, save=True)[1] if keep else None
+        dx, dwg, dwu, dwd = mf.gated_ffn_backward(dy, x, wg, wu, wd, act, saved=saved)
+        assert torch.isnan(dx).all()
+        rest = [i for i in range(190) if i != 77]
+        for t in (dwg, dwu, dwd.t()):
+            assert torch.isnan(t[:, 77]).all() and torch.isfinite(t[:, rest]).all()
+    assert mf.device_status() == 0
