@@ -200,9 +200,16 @@ __global__ void __launch_bounds__(kOrthThreads, 1)
             double total = 0.0;
             for (int r = 0; r < ranks; ++r)
                 total += ld_cluster_f64(mapa_shared(sums + kOrthWarps, r));
-            const float f = static_cast<float>(1.0 / (sqrt(total) + static_cast<double>(g.eps)));
+            // in two factors, a power of two and the rest: alone it leaves fp32's normal range where
+            // the norm is above 2^126
+            const double f = 1.0 / (sqrt(total) + static_cast<double>(g.eps));
+            const int e = static_cast<int>((__double_as_longlong(f) >> 52) & 0x7ff) - 1023;
+            const int half = max(-100, min(100, e / 2));
+            const float f1 = __int_as_float((127 + half) << 23);
+            const float f2 = static_cast<float>(
+                f * __longlong_as_double(static_cast<long long>(1023 - half) << 52));
 #pragma unroll
-            for (int j = 0; j < kOrthCols; ++j) x[j] *= f;
+            for (int j = 0; j < kOrthCols; ++j) x[j] = (x[j] * f1) * f2;
         }
         bool alive = true;  // a wait that gave up: finish without waiting, every barrier is met
         auto product_done = [&]() {

@@ -526,9 +526,10 @@ __global__ void __launch_bounds__(256) split_normalize_kernel(const double* sums
         if (static_cast<int>(threadIdx.x) < o) part[threadIdx.x] += part[threadIdx.x + o];
         __syncthreads();
     }
-    const float f = static_cast<float>(1.0 / (sqrt(part[0]) + static_cast<double>(eps)));
+    // in double: the factor alone leaves fp32's normal range where the norm is above 2^126
+    const double f = 1.0 / (sqrt(part[0]) + static_cast<double>(eps));
     float* q = inv + static_cast<long long>(blockIdx.x) * blocks;
-    for (int i = threadIdx.x; i < blocks; i += 256) q[i] *= f;
+    for (int i = threadIdx.x; i < blocks; i += 256) q[i] = static_cast<float>(q[i] * f);
 }
 
 // ---- activations of the gated block ----------------------------------------------------------

@@ -157,3 +157,23 @@ def test_what_ran_before_does_not_matter(cuda, shape):
         mf.orthogonalize(x)
         assert torch.equal(mf.orthogonalize(u), first)
     assert mf.device_status() == 0
+
+
+@pytest.mark.parametrize("shape", [(60, 100), (200, 400), (400, 200), (3, 100, 300), (2, 300, 140)])
+def test_norms_whose_reciprocal_leaves_fp32(cuda, shape):
+    """With eps = 0 a power of two in front of the matrix changes nothing, bit for bit, from
+    subnormal entries (norms below 2^-128) to the largest (norms above 2^128). Entries of ten bits
+    keep all of them as subnormals. At 2^-149 the block scale ends at 2^126 and leaves up to 511
+    2^-23 < 2^-14: exact, but subnormal in fp16, and a tensor product need not drop the same bits
+    of its sums for operands without a leading one; there the iteration's tolerance holds."""
+    g = torch.Generator(device="cuda").manual_seed(sum(shape))
+    u = torch.randint(-511, 512, shape, generator=g, device=cuda).float()
+    plain = mf.orthogonalize(u, eps=0.0)
+    close(plain, want(u, eps=0.0))
+    for power in (-149, -140, -120, 100, 118):
+        scaled = torch.ldexp(u.double(), torch.tensor(power, device=cuda)).float()
+        assert bool(torch.isfinite(scaled).all())
+        got = mf.orthogonalize(scaled, eps=0.0)
+        close(got, want(u, eps=0.0))
+        assert power == -149 or torch.equal(got, plain), power
+    assert mf.device_status() == 0
