@@ -25,8 +25,8 @@ constexpr int kRowsRingBytes = 65536;   // weights on their way: 8 KB per warp; 
 constexpr int kRowsSmem = kRowsXBytes + kRowsRingBytes;
 
 struct RowsArgs {
-    const float* x;          // element (r, k) at x[r*x_rs + k*x_cs]
-    long long x_rs, x_cs;
+    const float* x;          // element (r, k) at x[r*x_rs + k]
+    long long x_rs;
     const float* w0;         // the weights (gate), row stride ld0
     const float* w1;         // up
     long long ld0, ld1;
@@ -70,7 +70,7 @@ __device__ __forceinline__ void rows_stage_x(const RowsArgs& g, float* xs, int k
 #pragma unroll 4
     for (int i = threadIdx.x; i < depth * MT; i += 256) {
         const int r = i % MT, k = i / MT;
-        const float v = r < g.rows ? g.x[r * g.x_rs + (k0 + k) * g.x_cs] : 0.0f;
+        const float v = r < g.rows ? g.x[r * g.x_rs + (k0 + k)] : 0.0f;
         if constexpr (DUP == 2) {
             *reinterpret_cast<float2*>(xs + r * rs + k * ks) = make_float2(v, v);
         } else {

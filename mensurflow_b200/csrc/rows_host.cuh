@@ -119,7 +119,6 @@ int run_gated_rows(const mfk_gated_ffn_desc* d, float* y, int64_t ldy, const Dev
     mfk::RowsArgs g{};
     g.x = d->x;
     g.x_rs = d->x_rs;
-    g.x_cs = d->x_cs;
     g.w0 = d->w_gate;
     g.w1 = d->w_up;
     g.ld0 = tg ? d->w_gate_cs : d->w_gate_rs;
@@ -135,7 +134,6 @@ int run_gated_rows(const mfk_gated_ffn_desc* d, float* y, int64_t ldy, const Dev
     mfk::RowsArgs o{};
     o.x = h;
     o.x_rs = ldh;
-    o.x_cs = 1;
     o.w0 = d->w_down;
     o.ld0 = td ? d->w_down_cs : d->w_down_rs;
     o.rows = g.rows;

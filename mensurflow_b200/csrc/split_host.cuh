@@ -386,6 +386,7 @@ int run_gated_ffn(const mfk_gated_ffn_desc* d, float* y, int64_t ldy, float* sav
     if (d->rows > 0 && d->d > 0 && (y == nullptr || ldy < d->d)) return MFK_ERR_INVALID_ARGUMENT;
     if (d->rows == 0 || (d->d == 0 && saved == nullptr)) return MFK_OK;
     if (saved != nullptr && !aligned16(saved)) return MFK_ERR_INVALID_ARGUMENT;
+    if (d->d > 1 && d->x_cs != 1) return MFK_ERR_UNSUPPORTED;
     XWorkspace ws(stream);
     rc = current_device(&ws.dev, &ws.info);
     if (rc != MFK_OK) return rc;

@@ -165,3 +165,15 @@ def test_descriptor_layouts():
     assert ctypes.sizeof(_lib.GatedFfnDesc) == 4 * 24 + 24 + 8
     assert _lib.GatedFfnDesc.rows.offset == 96
     assert ctypes.sizeof(_lib.GatedFfnGrads) == 24 + 16 + 16 + 16 + 24
+
+
+@pytest.mark.parametrize("rows", [1, 5, 16, 17, 300])
+def test_rows_of_x_that_are_not_contiguous_are_refused(rows):
+    """However many rows: the few-rows form has no strided reads either."""
+    so, p = _lib.lib(), ctypes.c_void_p(4096)
+    for rs, cs in ((8, 2), (1, rows), (0, 0)):
+        if cs == 1:
+            continue
+        d = _lib.GatedFfnDesc(4096, rs, cs, 4096, 6, 1, 4096, 6, 1, 4096, 4, 1, rows, 4, 6, 0, 0)
+        assert so.mfk_gated_ffn_f32(ctypes.byref(d), p, 4, None, None) == _lib.MFK_ERR_UNSUPPORTED
+        assert so.mfk_gated_ffn_f32(ctypes.byref(d), p, 4, p, None) == _lib.MFK_ERR_UNSUPPORTED
