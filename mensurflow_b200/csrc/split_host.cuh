@@ -671,6 +671,7 @@ int run_orthogonalize(const float* u, int64_t batch, int64_t rows, int64_t cols,
             g.mb = g.nb = gram.rb;
             g.m = g.n = static_cast<int>(k);
             g.sym = 1;
+            g.alpha = 1.0f;
             g.o[0] = x_out(ws, gram);
             rc = x_product<mfk::kXSplit>(ws, g, depth, 0, batch);
             if (rc != MFK_OK) return rc;

@@ -88,7 +88,7 @@ struct XArgs {
     int m, n;              // output entries
     int tiles_m, tiles_n, splits, units, sym;
     int tiles;             // per matrix
-    float alpha, beta;     // acc * alpha + C * beta
+    float alpha, beta;     // acc * alpha + C * beta (kXF32 without C: acc)
     XOut c;                // C as a split matrix (beta != 0)
     float* out;            // fp32 output, row stride ld, batch stride out_bs
     long long ld, out_bs;
@@ -1092,6 +1092,9 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
                     }
                 }
                 cp_async_wait<0>();
+            } else if (EPI == kXSplit && g.alpha != 1.0f) {
+#pragma unroll
+                for (int j = 0; j < NB * 64; ++j) acc[j] *= g.alpha;
             }
         }
 

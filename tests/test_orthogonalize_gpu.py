@@ -177,3 +177,14 @@ def test_norms_whose_reciprocal_leaves_fp32(cuda, shape):
         close(got, want(u, eps=0.0))
         assert power == -149 or torch.equal(got, plain), power
     assert mf.device_status() == 0
+
+
+@pytest.mark.parametrize("shape", [(60, 100), (200, 400), (700, 300), (2, 1100, 1030)])
+@pytest.mark.parametrize("c", [(1.5, 0.0, -0.5), (0.0, 1.5, -0.5), (1.5, -0.5, 0.0),
+                               (1.25, 0.0, 0.0), (0.0, 0.0, 1.0), (0.0, 0.5, 0.0)])
+def test_coefficients_of_zero(cuda, shape, c):
+    g = torch.Generator(device="cuda").manual_seed(sum(shape))
+    u = torch.randn(*shape, generator=g, device=cuda)
+    for steps in (1, 3):
+        close(mf.orthogonalize(u, steps, c), want(u, steps, c))
+    assert mf.device_status() == 0
