@@ -137,6 +137,13 @@ int current_device(int* dev, DeviceInfo** info) {
     std::lock_guard<std::mutex> lock(g_mutex);
     DeviceInfo& d = g_devices[*dev];
     if (!d.ready) {
+        // A first call may be under capture: setting up the pool touches no stream, but in the other
+        // modes it ends this thread's capture.
+        struct Relaxed {
+            cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+            Relaxed() { cudaThreadExchangeStreamCaptureMode(&mode); }
+            ~Relaxed() { cudaThreadExchangeStreamCaptureMode(&mode); }
+        } relaxed;
         MFK_CUDA(cudaDeviceGetAttribute(&d.sm_count, cudaDevAttrMultiProcessorCount, *dev));
         MFK_CUDA(cudaDeviceGetAttribute(&d.major, cudaDevAttrComputeCapabilityMajor, *dev));
         MFK_CUDA(cudaDeviceGetAttribute(&d.minor, cudaDevAttrComputeCapabilityMinor, *dev));
