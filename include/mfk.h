@@ -352,8 +352,8 @@ int mfk_copy_peer(void* dst, int32_t dst_device, const void* src, int32_t src_de
  * the backward pass every matrix, have one per 128 x 128 block. Under one scale an entry keeps 22
  * bits or more while it is within 2^-17 of the largest, and an absolute error of 2^-39 of that one
  * below; dgate, dup and h of the backward pass, whose scales may be three powers of two larger,
- * within 2^-14, and 2^-36 below. A non-finite operand entry makes the results that depend on it non-finite (an infinity may
- * come out as NaN). Up to 16 rows without `saved` are plain fp32 sums.
+ * within 2^-14, and 2^-36 below. A non-finite operand entry makes the results that depend on it
+ * non-finite (an infinity may come out as NaN). Up to 16 rows without `saved` are plain fp32 sums.
  *
  * mfk_gated_ffn_f32: y has row stride ldy >= d. saved (optional, 16-byte aligned,
  * mfk_gated_ffn_saved_floats(rows, f) floats of device memory) receives gate and up for the
@@ -408,8 +408,8 @@ int mfk_gated_ffn_backward_f32(const mfk_gated_ffn_desc* desc, const mfk_gated_f
  * matrices of rows x cols: u at update + i*batch_stride with row stride row_stride and unit column
  * stride (any row stride), the result at out + i*out_batch_stride with row stride ld >= cols. out
  * must not overlap update. steps >= 1, eps >= 0 (a zero matrix with eps = 0 gives NaN). The norm
- * is summed in double; the products are computed as in mfk_gated_ffn_f32. No counterpart in the
- * reference. */
+ * is summed in double, and its reciprocal need not be an fp32 number; the products are computed as
+ * in mfk_gated_ffn_f32, with one scale per 128 x 128 block. No counterpart in the reference. */
 int mfk_orthogonalize_f32(const float* update, int64_t batch, int64_t rows, int64_t cols,
                           int64_t row_stride, int64_t batch_stride, float* out, int64_t ld,
                           int64_t out_batch_stride, int32_t steps, float a, float b, float c,
@@ -428,7 +428,9 @@ int mfk_orthogonalize_f32(const float* update, int64_t batch, int64_t rows, int6
  * whose id is `padding` take no part (negative: none is left out); an id outside [0, rows) that is
  * not `padding` takes no part either and sets MFK_DEVERR_INDEX. With rows = 0 nothing is done. The
  * sums are fp32, in an order that depends on the ids and sizes alone, so repeated calls give the
- * same bits. The workspace (16 bytes per token, n d / 2 bytes at most for partial rows) comes from the stream-ordered allocator. */
+ * same bits. The workspace comes from the stream-ordered allocator: about 16.5 bytes per token,
+ * rows / 8 bytes of marks, and 8 d bytes per window of 16 (few tokens) to 256 tokens for the
+ * partial rows of runs that cross windows. */
 int mfk_embedding_f32(const float* table, int64_t rows, int64_t d, int64_t ld, const void* ids,
                       int32_t id_bytes, int64_t n, float scale, float* out, int64_t ld_out,
                       void* stream);

@@ -48,9 +48,10 @@ from .ops import (  # noqa: F401
 )
 
 __all__ = [
-    "GatedSaved", "MfkError", "PackedB", "build", "add", "attention", "bias_add", "bias_grad", "contiguous",
-    "copy", "device_status", "div", "dot", "mul", "scal", "sub",
-    "embedding", "embedding_grad", "gated_ffn", "gated_ffn_backward", "gelu", "gemm", "gemm_prepacked", "gemm_strided_batched", "gemv", "get_default_precision",
-    "linear", "linear_backward", "log_softmax", "matmul", "matmul_backward", "matvec",
-    "orthogonalize", "pack_b", "relu", "set_default_precision", "softmax", "to", "where",
+    "GatedSaved", "MfkError", "PackedB", "build", "add", "attention", "bias_add", "bias_grad",
+    "contiguous", "copy", "device_status", "div", "dot", "mul", "scal", "sub", "embedding",
+    "embedding_grad", "gated_ffn", "gated_ffn_backward", "gelu", "gemm", "gemm_prepacked",
+    "gemm_strided_batched", "gemv", "get_default_precision", "linear", "linear_backward",
+    "log_softmax", "matmul", "matmul_backward", "matvec", "orthogonalize", "pack_b", "relu",
+    "set_default_precision", "softmax", "to", "where",
 ]

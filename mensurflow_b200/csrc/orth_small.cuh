@@ -200,8 +200,8 @@ __global__ void __launch_bounds__(kOrthThreads, 1)
             double total = 0.0;
             for (int r = 0; r < ranks; ++r)
                 total += ld_cluster_f64(mapa_shared(sums + kOrthWarps, r));
-            // in two factors, a power of two and the rest: alone it leaves fp32's normal range where
-            // the norm is above 2^126
+            // in two factors, a power of two and the rest: alone it leaves fp32's normal range
+            // where the norm is above 2^126
             const double f = 1.0 / (sqrt(total) + static_cast<double>(g.eps));
             const int e = static_cast<int>((__double_as_longlong(f) >> 52) & 0x7ff) - 1023;
             const int half = max(-100, min(100, e / 2));

@@ -122,7 +122,6 @@ bool x_source(XWorkspace& ws, mfk::XSources& list, XMat* out, const float* p, in
     s.bs = batch > 1 ? bs : 0;
     s.rows = static_cast<int>(out->rows);
     s.cols = static_cast<int>(out->cols);
-    s.batch = static_cast<int>(batch);
     s.rb = out->rb;
     s.cb = out->cb;
     s.by_row = by_row ? 1 : 0;
@@ -216,7 +215,7 @@ int x_slots(XWorkspace& ws, int kind, int cluster, int* slots) {
 // Time of a launch in SM cycles: whole waves of tiles, and the part of the epilogue that no product
 // hides. A chunk of 128 takes 24 MMAs, of 128 cycles for a pair's 256 x 256, which it reaches (its
 // 128 KB per CTA come at 42 bytes a cycle). One CTA's 128 x 128 would take 24 x 64, but 128 KB in
-// that time is more than an SM gets from L2: 2500 measured (4 to 50 chunks), and 4200 for 128 x 256.
+// that time is more than an SM gets from L2: 2500 measured (4 to 50 chunks), 4200 for 128 x 256.
 // Sharing a contraction costs 9000 cycles (128 x 128) or 17000 per wave (1024 x 1024 over a depth
 // of 1024: 15.6 us by clusters of 3 single CTAs, 24.5 us by clusters of 4 pairs).
 double x_cost(int64_t tiles, int slots, double chunk, int kc, double epilogue) {

@@ -325,8 +325,8 @@ __device__ __forceinline__ void store_split8(uint8_t* block, int chunk, int row,
 struct XSource {
     const float* src;      // rows x cols, unit column stride
     long long rs, bs;      // row stride, batch stride (elements)
-    int rows, cols, batch;
-    int rb, cb;            // blocks
+    int rows, cols;
+    int rb, cb;            // blocks of a matrix
     int vec;               // every row starts on 16 bytes
     int first;             // index of this matrix's first block in the launch
     uint8_t* data;
@@ -638,8 +638,8 @@ __device__ __forceinline__ void with_act(int act, F&& f) {
 // The largest |act'| over all inputs (GELU's is 1.1290): bounds the gate's gradient.
 constexpr float kXMaxSlope = 1.13f;
 
-// fp16 bits of 2^11: a block whose scale brought a bound into [2^14, 2^15) and whose largest |hi| is
-// below, or infinite, has a scale that is more than three powers of two off, or unknown.
+// fp16 bits of 2^11: a block whose scale brought a bound into [2^14, 2^15) and whose largest |hi|
+// is below, or infinite, has a scale that is more than three powers of two off, or unknown.
 constexpr uint32_t kXTight = 0x6800u;
 constexpr float kXMostScale = 8.507059173e37f;  // 2^126, the largest that split_scale gives
 
@@ -661,7 +661,7 @@ struct XConfig {
 };
 
 struct XUnit {
-    int z, tm, tn, s, c0, c1, tile;
+    int z, tm, tn, s, c0, c1;
 };
 
 template <int EPI>
@@ -674,7 +674,6 @@ __device__ __forceinline__ XUnit x_unit(const XArgs& g, int u) {
     XUnit w;
     const int t = u / g.splits;
     w.s = u - t * g.splits;
-    w.tile = t;
     w.z = t / g.tiles;
     int q = t - w.z * g.tiles;
     if (g.sym) {  // lower triangle, row by row
@@ -1270,14 +1269,14 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
             // acc: the gradient of h. The three outputs are stored under scales from bounds, the
             // largest over a block's rows of
             // |dgate| <= 1.13 max|dh| max|up|, |dup| <= max|dh| max|gate|, |h| <= max|gate| max|up|
-            // (the maxima over the row's 64 columns), and the largest |hi| is kept. On ordinary rows
-            // a bound is up to three powers of two too large, which leaves an entry its 22 bits down
-            // to 2^-14 of the largest. Where gates are saturated, act and act' are tiny and it can
-            // be any number too large (2^25 for SiLU at -20): such blocks are computed once more by
-            // the next launch (kXGatedAgain), which looks for their largest values first. (8192 x
-            // 4096 x 11008: 1800 us with bounds alone, 1835 so, and 5 for a next launch that finds
-            // nothing to do; 2070 in one launch that stores loose blocks twice, because a pair's 128
-            // sums a thread stay alive for that.)
+            // (the maxima over the row's 64 columns), and the largest |hi| is kept. On ordinary
+            // rows a bound is up to three powers of two too large, which leaves an entry its 22
+            // bits down to 2^-14 of the largest. Where gates are saturated, act and act' are tiny
+            // and it can be any number too large (2^25 for SiLU at -20): such blocks are computed
+            // once more by the next launch (kXGatedAgain), which looks for their largest values
+            // first. (8192 x 4096 x 11008: 1800 us with bounds alone, 1835 so, and 5 for a next
+            // launch that finds nothing to do; 2070 in one launch that stores loose blocks twice,
+            // because a pair's 128 sums a thread stay alive for that.)
             // A row without a gradient has no part in any sum over rows, whatever is in it: its
             // dgate, dup and h are zeros (as computed they would be 0 times gate and up, which need
             // not be finite there), and its size does not count.
