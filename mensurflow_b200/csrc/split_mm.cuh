@@ -1331,9 +1331,11 @@ __device__ __forceinline__ void x_epilogue(const XArgs& g, uint8_t* stages, uint
                     __half2 hi[3] = {};
 #pragma unroll
                     for (int e = 0; e < 3; ++e) {
+                        const uint32_t top = top_of[b * 3 + e];
                         float inv;
-                        split_scale(__uint_as_float(max(top_of[b * 3 + e], 1u)), sc[e], inv);
-                        if (pass == 1 && et == 0 && w.s == 0) g.o[e].inv[blk] = inv;
+                        split_scale(__uint_as_float(max(top, 1u)), sc[e], inv);
+                        if (pass == 1 && et == 0 && w.s == 0)
+                            g.o[e].inv[blk] = top != 0u ? inv : 1.0f;  // (a block of zeros)
                     }
                     with_act(g.act, [&](auto kind) {
 #pragma unroll
@@ -1477,6 +1479,7 @@ __global__ void __launch_bounds__(kXThreads, 1)
         work = __syncthreads_or(any) != 0;
     }
     if (!work) {
+        // straight to the end
     } else if (warp == 0) {
         if (lane == 0)
             x_producer<CG, NB, EPI>(g, &mk, &mm, stages, full, empty, rank, leader, first, step);
