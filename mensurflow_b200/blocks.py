@@ -236,8 +236,9 @@ def orthogonalize(update: torch.Tensor, steps: int = 5,
     are symmetric: only their lower halves are computed. Arithmetic as in ``gated_ffn``."""
     op = "orthogonalize"
     _require(update, op, "update", 2, at_least=True)
-    if not isinstance(steps, int) or isinstance(steps, bool) or steps < 1:
-        raise ValueError(f"{op}: steps must be a whole number of at least 1, got {steps!r}")
+    if not isinstance(steps, int) or isinstance(steps, bool) or not 1 <= steps < 2 ** 31:
+        raise ValueError(f"{op}: steps must be a whole number of at least 1 and below 2^31, "
+                         f"got {steps!r}")
     if len(coefficients) != 3:
         raise ValueError(f"{op}: coefficients must be (a, b, c)")
     if not eps >= 0:

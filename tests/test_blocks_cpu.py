@@ -177,3 +177,10 @@ def test_rows_of_x_that_are_not_contiguous_are_refused(rows):
         d = _lib.GatedFfnDesc(4096, rs, cs, 4096, 6, 1, 4096, 6, 1, 4096, 4, 1, rows, 4, 6, 0, 0)
         assert so.mfk_gated_ffn_f32(ctypes.byref(d), p, 4, None, None) == _lib.MFK_ERR_UNSUPPORTED
         assert so.mfk_gated_ffn_f32(ctypes.byref(d), p, 4, p, None) == _lib.MFK_ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("steps", [2 ** 31, 2 ** 32, 2 ** 32 + 5])
+def test_steps_beyond_32_bits_are_refused(steps):
+    """The entry point's count has 32 bits: 2^32 + 5 would be 5."""
+    with pytest.raises(ValueError, match="steps"):
+        mf.orthogonalize(torch.ones(3, 4), steps)
