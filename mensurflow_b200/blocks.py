@@ -319,6 +319,8 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, rows: int, scale: floa
         raise ValueError(f"{op}: grad {tuple(grad.shape)} does not fit ids {tuple(ids.shape)}")
     if not isinstance(rows, int) or isinstance(rows, bool) or rows < 0:
         raise ValueError(f"{op}: rows must be a whole number of at least 0, got {rows!r}")
+    if padding is not None and (not isinstance(padding, int) or isinstance(padding, bool)):
+        raise ValueError(f"{op}: padding must be a whole number, got {padding!r}")
     if padding is not None and not 0 <= padding < rows:
         raise ValueError(f"{op}: padding {padding} is outside the table of {rows} rows")
     _kernel_for(op, grad)

@@ -184,3 +184,9 @@ def test_steps_beyond_32_bits_are_refused(steps):
     """The entry point's count has 32 bits: 2^32 + 5 would be 5."""
     with pytest.raises(ValueError, match="steps"):
         mf.orthogonalize(torch.ones(3, 4), steps)
+
+
+@pytest.mark.parametrize("padding", [1.5, 2.0, "1", True, [1]])
+def test_padding_that_is_no_whole_number_is_refused(padding):
+    with pytest.raises(ValueError, match="padding"):
+        mf.embedding_grad(torch.ones(3, 4), torch.zeros(3, dtype=torch.int64), 5, padding=padding)
